@@ -429,6 +429,103 @@ TOPS_API int tops_gla_gate_logsigmoid_fwd(int64_t n, int32_t dtype, float normal
 TOPS_API int tops_gla_gate_logsigmoid_bwd(int64_t n, int32_t dtype, float normalizer, float clamp_min,
                                           int32_t has_clamp, const void* x, const float* dy, void* dx, void* stream);
 
+/* ---- causal short convolution, prompts and single tokens ------------------------
+ * p_t = bias + sum_{j<W} w[:, j] x_{t-W+1+j},  y = p (activation 0) or p sigmoid(p) (1).
+ * x [B,T,D] with strides in elements (batch, row; channels contiguous); w [D,W] and bias [D] in
+ * w_dtype (= dtype or TOPS_F32); W in 2..4; initial_state / final_state [N,D,W-1] (dtype, last
+ * column = newest input) or NULL; y [B,T,D] dense.  With cu_seqlens (device [N+1], B == 1) the
+ * rows are N packed sequences; the offsets are not read on the host: the kernels clamp them to
+ * [0, T], and rows that no sequence covers give y = 0 and no gradient.  Replaces
+ * ShortConvolution's conv1d (tops/modules/convolution.py:6). */
+typedef struct tops_gla_conv_args {
+  int32_t B, T, D, W, N, dtype, w_dtype, activation;
+  const int32_t* cu_seqlens;
+  const void* x; int64_t x_stride_b, x_stride_t;
+  const void* w; const void* bias; const void* initial_state;
+  void* y; void* final_state;
+} tops_gla_conv_args;
+
+/* Backward: dx [B,T,D] dense; dw [D,W], dbias [D] (w_dtype), dstate [N,D,W-1] (dtype), each NULL if
+ * not wanted; dfinal = gradient of final_state or NULL. */
+typedef struct tops_gla_conv_bwd_args {
+  tops_gla_conv_args f;
+  const void* dy; int64_t dy_stride_b, dy_stride_t;
+  const void* dfinal;
+  void* dx; void* dw; void* dbias; void* dstate;
+  void* workspace; size_t workspace_bytes;
+} tops_gla_conv_bwd_args;
+
+TOPS_API int tops_gla_causal_conv_fwd(const tops_gla_conv_args* a, void* stream);
+TOPS_API size_t tops_gla_causal_conv_bwd_workspace_size(const tops_gla_conv_bwd_args* a);
+TOPS_API int tops_gla_causal_conv_bwd(const tops_gla_conv_bwd_args* a, void* stream);
+/* One token of each of B rows (T == 1): final_state may be initial_state itself. */
+TOPS_API int tops_gla_causal_conv_step(const tops_gla_conv_args* a, void* stream);
+
+/* ---- selective state space scan, prompts and single tokens ------------------------
+ * delta = dt + dt_bias, through softplus if `softplus`;  h_t = exp(delta A) h_{t-1} + delta x B_t;
+ * y = C_t . h_t + skip x;  out = y silu(z).
+ * x, dt, z [B,T,D] and Bm, Cm [B,T,G,N] in dtype, strides in elements (batch, row; the rest
+ * contiguous); A [D,N], skip [D], dt_bias [D], h0 / ht [S,D,N] fp32; skip, dt_bias, z, h0, ht may be
+ * NULL; N in 1..64; G divides D.  cu_seqlens as in the convolution (S sequences; S == B without).
+ * `states` (tops_gla_ssm_scan_states_size() bytes, or NULL) keeps what the backward starts from. */
+typedef struct tops_gla_scan_args {
+  int32_t B, T, D, N, G, S, dtype, softplus;
+  const int32_t* cu_seqlens;
+  const void* x; const void* dt; const void* z; const void* Bm; const void* Cm;
+  int64_t x_strides[2], dt_strides[2], z_strides[2], b_strides[2], c_strides[2];
+  const float* A; const float* skip; const float* dt_bias; const float* h0;
+  void* y; float* ht; float* states;
+  void* workspace; size_t workspace_bytes;
+} tops_gla_scan_args;
+
+/* Backward: dx, ddt, dz [B,T,D] and dB, dC [B,T,G,N] dense (dtype); dA [D,N], dskip [D],
+ * ddt_bias [D], dh0 [S,D,N] fp32, each of the last four NULL if not wanted.  `f.states` from the
+ * forward; f.y, f.ht and f.workspace are not used. */
+typedef struct tops_gla_scan_bwd_args {
+  tops_gla_scan_args f;
+  const void* dout; int64_t dout_strides[2];
+  const float* dht;
+  void* dx; void* ddt; void* dz; void* dB; void* dC;
+  float* dA; float* dskip; float* ddt_bias; float* dh0;
+  void* workspace; size_t workspace_bytes;
+} tops_gla_scan_bwd_args;
+
+TOPS_API size_t tops_gla_ssm_scan_states_size(const tops_gla_scan_args* a);
+TOPS_API size_t tops_gla_ssm_scan_fwd_workspace_size(const tops_gla_scan_args* a);
+TOPS_API int tops_gla_ssm_scan_fwd(const tops_gla_scan_args* a, void* stream);
+TOPS_API size_t tops_gla_ssm_scan_bwd_workspace_size(const tops_gla_scan_bwd_args* a);
+TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream);
+/* One token of each of B rows (T == 1, h0 and ht required; ht may be h0 itself). */
+TOPS_API int tops_gla_ssm_scan_step(const tops_gla_scan_args* a, void* stream);
+
+/* ---- norm of queries and keys with the position rotation --------------------------
+ * Per head row: n = x / sqrt(mean x^2 + eps) * weight (weight [K] in w_dtype, or NULL); the first R
+ * elements are rotated in pairs (i, i + R/2), or (2i, 2i + 1) if `interleaved`, by the row's position:
+ * tables [table_rows, R/2] fp32 of cosines and sines; positions [B,T] int32 or int64 (batch stride
+ * given, 0 = shared by all) or NULL = 0..T-1.  A position outside the tables gives NaN in the rotated
+ * part.  q [B,T,H,K], k [B,T,HK,K] with strides (batch, row, head); outputs dense; K <= 256. */
+typedef struct tops_gla_qk_norm_args {
+  int32_t B, T, H, HK, K, R, dtype, w_dtype, interleaved, positions_int64, table_rows;
+  float eps;
+  const void* q; const void* k; int64_t q_strides[3], k_strides[3];
+  const void* q_weight; const void* k_weight;
+  const float* cos_table; const float* sin_table;
+  const void* positions; int64_t positions_stride_b;
+  void* q_out; void* k_out;
+} tops_gla_qk_norm_args;
+
+/* Backward: dq, dk dense (dtype); dq_weight, dk_weight [K] (w_dtype) or NULL. */
+typedef struct tops_gla_qk_norm_bwd_args {
+  tops_gla_qk_norm_args f;
+  const void* dq_out; const void* dk_out; int64_t dq_out_strides[3], dk_out_strides[3];
+  void* dq; void* dk; void* dq_weight; void* dk_weight;
+  void* workspace; size_t workspace_bytes;
+} tops_gla_qk_norm_bwd_args;
+
+TOPS_API int tops_gla_qk_norm_rotary_fwd(const tops_gla_qk_norm_args* a, void* stream);
+TOPS_API size_t tops_gla_qk_norm_rotary_bwd_workspace_size(const tops_gla_qk_norm_bwd_args* a);
+TOPS_API int tops_gla_qk_norm_rotary_bwd(const tops_gla_qk_norm_bwd_args* a, void* stream);
+
 /* ---- XLA custom calls (JAX frontend) ---------------------------------------
  * Status-returning legacy custom-call signature used by jax custom_call lowering:
  * (cudaStream_t, void** buffers, const char* opaque, size_t opaque_len,

@@ -1,0 +1,93 @@
+// Element access of the kernels that take every storage type with strides: vectors of V
+// elements of T in as few aligned 16-byte accesses as V allows, fp32 arithmetic between.
+#pragma once
+
+#include "common.cuh"
+
+namespace tops {
+
+template <typename T, int V>
+struct Vx {
+  static constexpr int BYTES = V * (int)sizeof(T);
+  static constexpr int UNIT = BYTES >= 16 ? 16 : BYTES;  // one access
+  static __device__ __forceinline__ void load(const T* p, float (&r)[V]) {
+    alignas(16) T raw[V];
+    load_raw(p, raw);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = to_f<T>(raw[i]);
+  }
+  static __device__ __forceinline__ void load_raw(const T* p, T (&raw)[V]) {
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i)
+        reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else if constexpr (BYTES == 8) {
+      *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) raw[i] = p[i];
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&r)[V]) {
+    alignas(16) T raw[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) raw[i] = from_f<T>(r[i]);
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(raw)[i];
+    } else if constexpr (BYTES == 8) {
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(raw);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[i] = raw[i];
+    }
+  }
+};
+
+// element i of a small parameter tensor stored in `dtype` (enum tops_dtype)
+__device__ __forceinline__ float load_param(const void* p, int dtype, int64_t i) {
+  if (dtype == TOPS_F32) return static_cast<const float*>(p)[i];
+  if (dtype == TOPS_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float v) {
+  if (dtype == TOPS_F32) static_cast<float*>(p)[i] = v;
+  else if (dtype == TOPS_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+__device__ __forceinline__ float fast_sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+// ---------------------------------------------------------------------------
+// packed sequences: rows [cu[n], cu[n+1]) of one axis of T rows.  The offsets lie on the
+// device and are not read by the host, so every value is clamped to the axis here: wrong
+// offsets give wrong rows, never an access out of range.  A row that no sequence covers
+// belongs to none (n = -1).
+// ---------------------------------------------------------------------------
+struct SeqAt {
+  int n, s, e;
+};
+
+__device__ __forceinline__ SeqAt seq_at(const int32_t* __restrict__ cu, int N, int T, int t) {
+  int lo = 0, hi = N - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(cu + mid) <= t) lo = mid; else hi = mid - 1;
+  }
+  SeqAt q{lo, max(__ldg(cu + lo), 0), min(__ldg(cu + lo + 1), T)};
+  if (t < q.s || t >= q.e) q.n = -1;
+  return q;
+}
+
+inline int sm_count() {
+  int dev = 0, n = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+inline bool dtype_known(int d) { return d == TOPS_F32 || d == TOPS_BF16 || d == TOPS_F16; }
+inline int dtype_bytes(int d) { return d == TOPS_F32 ? 4 : 2; }
+inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+}  // namespace tops

@@ -82,6 +82,52 @@ class P2PArgs(C.Structure):
                 ("own_region", C.c_void_p), ("timeout_ms", C.c_int32)]
 
 
+class ConvArgs(C.Structure):
+    _fields_ = [("B", C.c_int32), ("T", C.c_int32), ("D", C.c_int32), ("W", C.c_int32), ("N", C.c_int32),
+                ("dtype", C.c_int32), ("w_dtype", C.c_int32), ("activation", C.c_int32), ("cu_seqlens", C.c_void_p),
+                ("x", C.c_void_p), ("x_stride_b", C.c_int64), ("x_stride_t", C.c_int64), ("w", C.c_void_p),
+                ("bias", C.c_void_p), ("initial_state", C.c_void_p), ("y", C.c_void_p), ("final_state", C.c_void_p)]
+
+
+class ConvBwdArgs(C.Structure):
+    _fields_ = [("f", ConvArgs), ("dy", C.c_void_p), ("dy_stride_b", C.c_int64), ("dy_stride_t", C.c_int64),
+                ("dfinal", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
+                ("dstate", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class ScanArgs(C.Structure):
+    _fields_ = [("B", C.c_int32), ("T", C.c_int32), ("D", C.c_int32), ("N", C.c_int32), ("G", C.c_int32),
+                ("S", C.c_int32), ("dtype", C.c_int32), ("softplus", C.c_int32), ("cu_seqlens", C.c_void_p),
+                ("x", C.c_void_p), ("dt", C.c_void_p), ("z", C.c_void_p), ("Bm", C.c_void_p), ("Cm", C.c_void_p),
+                ("x_strides", C.c_int64 * 2), ("dt_strides", C.c_int64 * 2), ("z_strides", C.c_int64 * 2),
+                ("b_strides", C.c_int64 * 2), ("c_strides", C.c_int64 * 2), ("A", C.c_void_p), ("skip", C.c_void_p),
+                ("dt_bias", C.c_void_p), ("h0", C.c_void_p), ("y", C.c_void_p), ("ht", C.c_void_p),
+                ("states", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class ScanBwdArgs(C.Structure):
+    _fields_ = [("f", ScanArgs), ("dout", C.c_void_p), ("dout_strides", C.c_int64 * 2), ("dht", C.c_void_p),
+                ("dx", C.c_void_p), ("ddt", C.c_void_p), ("dz", C.c_void_p), ("dB", C.c_void_p), ("dC", C.c_void_p),
+                ("dA", C.c_void_p), ("dskip", C.c_void_p), ("ddt_bias", C.c_void_p), ("dh0", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class QKNormArgs(C.Structure):
+    _fields_ = [("B", C.c_int32), ("T", C.c_int32), ("H", C.c_int32), ("HK", C.c_int32), ("K", C.c_int32),
+                ("R", C.c_int32), ("dtype", C.c_int32), ("w_dtype", C.c_int32), ("interleaved", C.c_int32),
+                ("positions_int64", C.c_int32), ("table_rows", C.c_int32), ("eps", C.c_float), ("q", C.c_void_p),
+                ("k", C.c_void_p), ("q_strides", C.c_int64 * 3), ("k_strides", C.c_int64 * 3),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("cos_table", C.c_void_p),
+                ("sin_table", C.c_void_p), ("positions", C.c_void_p), ("positions_stride_b", C.c_int64),
+                ("q_out", C.c_void_p), ("k_out", C.c_void_p)]
+
+
+class QKNormBwdArgs(C.Structure):
+    _fields_ = [("f", QKNormArgs), ("dq_out", C.c_void_p), ("dk_out", C.c_void_p), ("dq_out_strides", C.c_int64 * 3),
+                ("dk_out_strides", C.c_int64 * 3), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dq_weight", C.c_void_p),
+                ("dk_weight", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 IPC_HANDLE_BYTES = 64
 VP, I32, F32C = C.c_void_p, C.c_int32, C.c_float
 SIGNATURES = {
@@ -146,6 +192,19 @@ SIGNATURES = {
     "tops_gla_p2p_combine": (C.c_int, [C.POINTER(P2PArgs), VP]),
     "tops_gla_chunk_fwd_span_begin_p2p": (C.c_int, [C.POINTER(ChunkFwdArgs), VP, C.POINTER(P2PArgs), VP]),
     "tops_gla_chunk_bwd_span_begin_p2p": (C.c_int, [C.POINTER(ChunkBwdArgs), VP, C.POINTER(P2PArgs), VP]),
+    "tops_gla_causal_conv_fwd": (C.c_int, [C.POINTER(ConvArgs), VP]),
+    "tops_gla_causal_conv_bwd_workspace_size": (C.c_size_t, [C.POINTER(ConvBwdArgs)]),
+    "tops_gla_causal_conv_bwd": (C.c_int, [C.POINTER(ConvBwdArgs), VP]),
+    "tops_gla_causal_conv_step": (C.c_int, [C.POINTER(ConvArgs), VP]),
+    "tops_gla_ssm_scan_states_size": (C.c_size_t, [C.POINTER(ScanArgs)]),
+    "tops_gla_ssm_scan_fwd_workspace_size": (C.c_size_t, [C.POINTER(ScanArgs)]),
+    "tops_gla_ssm_scan_fwd": (C.c_int, [C.POINTER(ScanArgs), VP]),
+    "tops_gla_ssm_scan_bwd_workspace_size": (C.c_size_t, [C.POINTER(ScanBwdArgs)]),
+    "tops_gla_ssm_scan_bwd": (C.c_int, [C.POINTER(ScanBwdArgs), VP]),
+    "tops_gla_ssm_scan_step": (C.c_int, [C.POINTER(ScanArgs), VP]),
+    "tops_gla_qk_norm_rotary_fwd": (C.c_int, [C.POINTER(QKNormArgs), VP]),
+    "tops_gla_qk_norm_rotary_bwd_workspace_size": (C.c_size_t, [C.POINTER(QKNormBwdArgs)]),
+    "tops_gla_qk_norm_rotary_bwd": (C.c_int, [C.POINTER(QKNormBwdArgs), VP]),
     "tops_gla_xla_chunk_fwd": (None, [VP, VP, C.c_char_p, C.c_size_t, VP]),
     "tops_gla_xla_chunk_bwd": (None, [VP, VP, C.c_char_p, C.c_size_t, VP]),
     "tops_gla_xla_recurrent_fwd": (None, [VP, VP, C.c_char_p, C.c_size_t, VP]),

@@ -1,0 +1,103 @@
+"""Argument handling shared by the operators that take strided rows and packed sequences
+(``causal_conv1d``, ``selective_scan``, ``qk_norm_rotary`` and their single-token forms)."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _C
+
+_NOTHING = contextlib.nullcontext()
+
+
+def check_cuda(op: str, first: torch.Tensor, **others) -> None:
+    """``first`` and every other given tensor lie on one CUDA device."""
+    if not first.is_cuda:
+        raise RuntimeError(f"{op} needs CUDA tensors (the kernels are the only implementation)")
+    if first.dtype not in _C._DTYPE:
+        raise TypeError(f"{op}: unsupported dtype {first.dtype} (float32, bfloat16 or float16)")
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{op}: {name} is on {t.device}, expected {first.device}")
+
+
+def check_like(op: str, name: str, t: torch.Tensor | None, shape: tuple, dtype: torch.dtype) -> None:
+    if t is None:
+        return
+    assert tuple(t.shape) == tuple(shape), f"{op}: expected {name} shape {tuple(shape)}, got {tuple(t.shape)}"
+    if t.dtype != dtype:
+        raise TypeError(f"{op}: {name} must be {dtype}, got {t.dtype}")
+
+
+def no_grad_only(op: str, other: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op} has no gradient: call {other}, or this under torch.no_grad()")
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def rows(t: torch.Tensor | None, inner: int = 1) -> torch.Tensor | None:
+    """``t`` itself where its last ``inner`` dims are dense, else a contiguous copy."""
+    if t is None or t.is_contiguous():
+        return t
+    want = 1
+    for i in range(1, inner + 1):
+        if t.shape[-i] != 1 and t.stride(-i) != want:
+            return t.contiguous()
+        want *= t.shape[-i]
+    return t
+
+
+def sequences(op: str, cu_seqlens, B: int, T: int, device) -> tuple[int, torch.Tensor | None]:
+    """(number of sequences, device int32 offsets or None).
+
+    Host offsets (list or CPU tensor) are checked and copied to the device.  Offsets that lie on the
+    device are used as they are, without a read on the host: such a call can be captured into a CUDA
+    graph and replayed with other offsets.  The kernels clamp them to [0, T]; rows behind the last
+    sequence give zeros."""
+    if cu_seqlens is None:
+        return B, None
+    assert B == 1, f"{op}: batch size must be 1 when using cu_seqlens, got {B}"
+    if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda:
+        assert cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2, f"{op}: cu_seqlens must be [N + 1] with N >= 1"
+        if cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{op}: cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
+        if cu_seqlens.device != device:
+            raise RuntimeError(f"{op}: cu_seqlens is on {cu_seqlens.device}, expected {device}")
+        return cu_seqlens.numel() - 1, cu_seqlens.to(torch.int32).contiguous()
+    cu = [int(c) for c in (cu_seqlens.tolist() if isinstance(cu_seqlens, torch.Tensor) else cu_seqlens)]
+    assert len(cu) >= 2 and cu[0] == 0 and cu[-1] == T, f"{op}: cu_seqlens must run from 0 to T={T}, got {cu}"
+    assert all(b >= a for a, b in zip(cu, cu[1:])), f"{op}: cu_seqlens must be non-decreasing"
+    return len(cu) - 1, torch.tensor(cu, dtype=torch.int32, device=device)
+
+
+def state_target(op: str, state: torch.Tensor, out: torch.Tensor | None, *reads) -> tuple:
+    """(state to read, tensor to write): ``out`` may be ``state`` itself; any other overlap with
+    what the call reads is refused."""
+    if out is None:
+        state = state.contiguous()
+        return state, torch.empty_like(state)
+    check_like(op, "state_out", out, state.shape, state.dtype)
+    if out.device != state.device:
+        raise RuntimeError(f"{op}: state_out is on {out.device}, expected {state.device}")
+    assert out.is_contiguous(), f"{op}: state_out must be contiguous"
+    a, n = out.data_ptr(), out.numel() * out.element_size()
+    same = state.data_ptr() == a and state.is_contiguous()
+    for t in reads if same else (state, *reads):
+        if t is not None and t.numel() and n:
+            last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+            if t.data_ptr() < a + n and a < t.data_ptr() + (last + 1) * t.element_size():
+                raise ValueError(f"{op}: state_out overlaps a tensor that the call reads")
+    return (state if same else state.contiguous()), out
+
+
+def on_device(t: torch.Tensor):
+    """The launches of a call go to its tensors' device, whatever the current one is."""
+    return _NOTHING if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def workspace(nbytes: int, t: torch.Tensor) -> torch.Tensor | None:
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=t.device) if nbytes else None
