@@ -1,0 +1,334 @@
+// Selective state space scan.  Per channel d with N states, delta = softplus(dt + bias) or dt + bias:
+//   h_t[n] = exp(delta_t A[d, n]) h_{t-1}[n] + delta_t x_t B_t[n],   y_t = sum_n C_t[n] h_t[n] + D x_t,
+//   out = y silu(z)          (B, C shared by the D / G channels of a group)
+// Backward, with dy = dout silu(z) and g_t = C_t dy_t + a_{t+1} g_{t+1} (the gradient of h_t):
+//   dC_t = sum_d dy h,  dB_t = sum_d g delta x,  dx = delta sum_n g B + D dy,
+//   ddelta = x sum_n g B + sum_n A a g h_{t-1},  dA = sum_t delta a g h_{t-1},  dh0 = a_1 g_1
+//
+// One exponential per (row, channel, state): at N = 16 the exponential unit (16 a clock and SM) bounds the
+// forward at twice the time that its bytes take, and instruction issue the backward.  So:
+//  * a thread owns CH channels x NT states and keeps their states, A and gradients in registers over all
+//    rows; LN lanes share a channel and the other lanes are other channels;
+//  * what a row needs once per channel (delta, delta x, dy) or once per state (B, C) is computed once per
+//    block, a tile of rows ahead, into shared memory; the tile's elementwise work (softplus, gates,
+//    rounding, 8- or 16-byte accesses) is spread over all threads, its loads issued one tile early;
+//  * sums over the lanes of a channel (y, and the backward's) and over channels (dB, dC) are folded for
+//    several rows at a time, so that each exchange halves the values that a lane still carries;
+//  * arithmetic on state pairs is packed (fma.rn.f32x2), which halves its issue slots.
+// Where B x D is too small for all SMs, the rows are split into segments: a first pass gives each segment's
+// decay and its state from zero, a small kernel chains them, and the main pass starts every segment from its
+// own state.  That costs the exponentials twice.
+#pragma once
+
+#include <algorithm>
+
+#include "rowtypes.cuh"
+
+namespace tops {
+namespace ssm {
+
+constexpr int CK = 16;  // rows between saved states = rows of a backward tile
+
+struct P {
+  int B, T, D, N, G, S, softplus;
+  const int32_t* cu;
+  const void *x, *dt, *z, *bm, *cm;
+  int64_t xs[2], ds[2], zs[2], bs[2], cs[2];
+  const float *A, *skip, *bias, *h0;
+  void* y;
+  float *ht, *states;
+  int vx, vd, vz, vb, vc, vy, vo, vg;  // four elements of that tensor may be read (written) at once
+  // segments of the rows
+  int seg, nseg;
+  float* carry;   // [B][nseg][D][N]: state (gradient) of a segment from zero, then the one it starts from
+  float* sdelta;  // [B][nseg][D]: sum of delta over a segment
+  int* broken;    // [nseg]: a sequence begins (ends) in the segment: nothing passes through it
+  // backward
+  const void* dout;
+  int64_t os[2];
+  const float* dht;
+  void *dx, *ddt, *dz;
+  float* pbc;   // [G][parts][B T][2][N]: dB, dC of one part of a group's channels
+  int parts;
+  float* pa;    // [B nseg][D][N]: dA of one segment
+  float* pd;    // [B nseg][2][D]: dD, dbias of one segment
+  float* dh0;
+};
+
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
+// ex2.approx errs by -2e-8 on average where decays lie (against 64 bits, arguments -1 .. -0.002), and a state's
+// error is that times the rows it remembers: the exponent's multiply-add takes the mean error back.
+constexpr float kEx2Mean = 2.0e-8f * kLog2e;
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
+// exp(delta A) of a pair, A given times log2(e)
+__device__ __forceinline__ float2 decay2(float delta, float2 A) {
+  const float2 e = fma2(dup(delta), A, dup(kEx2Mean));
+  return make_float2(ex2(e.x), ex2(e.y));
+}
+
+__device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1pf(__expf(v)); }
+
+// Sums of V values over the L lanes that differ in bits m0, 2 m0, ... of the lane: as long as a lane carries
+// several, an exchange halves them.  Returns the first index of the V >> log2(L) (at least one) that this lane holds.
+template <int V, int L, int M0>
+__device__ __forceinline__ int fold(float (&v)[V], int lane) {
+  int off = 0;
+  int cnt = V;
+#pragma unroll
+  for (int m = M0; m < L * M0; m <<= 1) {
+    const bool up = lane & m;
+    if (cnt > 1) {
+      cnt >>= 1;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i)
+        if (i < cnt) {
+          const float send = up ? v[i] : v[i + cnt], keep = up ? v[i + cnt] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+        }
+      if (up) off += cnt;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
+    }
+  }
+  return off;
+}
+
+// four elements of T (those at `valid` and beyond are zero)
+template <typename T>
+struct Quad {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ void quad_load(const T* p, bool vec, int valid, Quad<T>& q) {
+  if (vec && valid >= 4) {
+    alignas(16) T raw[4];
+    Vx<T, 4>::load_raw(p, raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q.v[i] = raw[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q.v[i] = i < valid ? p[i] : from_f<T>(0.f);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void quad_store(T* p, bool vec, int valid, const float (&r)[4]) {
+  if (vec && valid >= 4) {
+    Vx<T, 4>::store(p, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < valid) p[i] = from_f<T>(r[i]);
+  }
+}
+
+// NT states of one channel in global memory (those at N and beyond are not there)
+template <int NT>
+__device__ __forceinline__ void states_load(const float* p, int n0, int N, float2 (&h)[NT / 2]) {
+#pragma unroll
+  for (int i = 0; i < NT / 2; ++i)
+    h[i] = make_float2(n0 + 2 * i < N ? p[n0 + 2 * i] : 0.f, n0 + 2 * i + 1 < N ? p[n0 + 2 * i + 1] : 0.f);
+}
+template <int NT>
+__device__ __forceinline__ void states_store(float* p, int n0, int N, const float2 (&h)[NT / 2]) {
+  if (NT == 4 && N % 4 == 0) {
+    if (n0 < N) *reinterpret_cast<float4*>(p + n0) = make_float4(h[0].x, h[0].y, h[NT / 2 - 1].x, h[NT / 2 - 1].y);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < NT / 2; ++i) {
+    if (n0 + 2 * i < N) p[n0 + 2 * i] = h[i].x;
+    if (n0 + 2 * i + 1 < N) p[n0 + 2 * i + 1] = h[i].y;
+  }
+}
+template <int NT>
+__device__ __forceinline__ void pairs_load(const float* p, float2 (&v)[NT / 2]) {
+  if constexpr (NT == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = make_float2(f.x, f.y);
+    v[1] = make_float2(f.z, f.w);
+  } else {
+    v[0] = *reinterpret_cast<const float2*>(p);
+  }
+}
+
+// what a row is to packed sequences
+enum { kFirst = 1, kLast = 2, kNone = 4 };
+__device__ __forceinline__ int row_flags(const P& p, int t, int& n) {
+  const SeqAt q = seq_at(p.cu, p.S, p.T, t);
+  n = q.n;
+  return q.n < 0 ? kNone : (t == q.s ? kFirst : 0) | (t == q.e - 1 ? kLast : 0);
+}
+
+// Chains the segments: slot k becomes what segment k starts from.  Forward: slot 0 is not read by the main pass
+// (segment 0's own pass began with h0).  Backward: from the last segment, which starts from dht (packed: zero).
+template <bool BACK>
+__global__ void __launch_bounds__(128) k_scan_chain(const P p) {
+  const int64_t dn = (int64_t)p.D * p.N, i = (int64_t)blockIdx.x * 128 + threadIdx.x;
+  const int b = blockIdx.y;
+  if (i >= dn) return;
+  const float A = p.A[i] * kLog2e;
+  float c = BACK && p.dht && !p.cu ? p.dht[b * dn + i] : 0.f;
+  for (int s = 0; s < p.nseg; ++s) {
+    const int k = BACK ? p.nseg - 1 - s : s;
+    if (s == p.nseg - 1) {
+      p.carry[((int64_t)b * p.nseg + k) * dn + i] = c;
+      break;
+    }
+    const int64_t at = ((int64_t)b * p.nseg + k) * dn + i;
+    const float own = p.carry[at];
+    p.carry[at] = c;
+    // segment 0 forward began with h0 itself
+    if ((p.cu && p.broken[k]) || (!BACK && s == 0)) c = own;
+    else c = fmaf(ex2(A * p.sdelta[((int64_t)b * p.nseg + k) * p.D + i / p.N]), c, own);
+  }
+}
+
+// Packed sequences without rows: their final state is their initial one (and its gradient the
+// final state's).
+static __global__ void k_scan_empty(int S, int T, int64_t DN, const int32_t* __restrict__ cu, const float* __restrict__ from,
+                             float* __restrict__ to) {
+  const int n = blockIdx.y;
+  if (min(cu[n + 1], T) > max(cu[n], 0)) return;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < DN; i += (int64_t)gridDim.x * blockDim.x)
+    to[n * DN + i] = from ? from[n * DN + i] : 0.f;
+}
+
+constexpr int kMinSegment = 128, kFwdBlocks = 148, kBwdBlocks = 148;
+
+inline int check(const tops_gla_scan_args* a) {
+  TOPS_CHECK_ARG(a != nullptr, "ssm_scan: args is NULL");
+  TOPS_CHECK_ARG(a->B >= 0 && a->T >= 0 && a->D > 0 && a->S >= 0, "ssm_scan: negative or zero dimension");
+  TOPS_CHECK_ARG(a->G > 0 && a->D % a->G == 0, "ssm_scan: D must be a multiple of G");
+  if (a->G > 65535) return fail(TOPS_ERR_UNSUPPORTED, "ssm_scan: at most 65535 groups");
+  if (a->N < 1 || a->N > 64) return fail(TOPS_ERR_UNSUPPORTED, "ssm_scan: a channel must have 1 to 64 states");
+  TOPS_CHECK_ARG(dtype_known(a->dtype), "ssm_scan: unknown dtype");
+  if (a->B > 65535) return fail(TOPS_ERR_UNSUPPORTED, "ssm_scan: at most 65535 batch rows");
+  if (a->cu_seqlens) {
+    TOPS_CHECK_ARG(a->B == 1, "ssm_scan: cu_seqlens requires B == 1");
+    TOPS_CHECK_ARG(a->S >= 1 && a->S <= 65535, "ssm_scan: cu_seqlens requires 1 to 65535 sequences");
+  } else {
+    TOPS_CHECK_ARG(a->S == a->B, "ssm_scan: S must equal B without cu_seqlens");
+  }
+  return TOPS_OK;
+}
+
+inline P params(const tops_gla_scan_args* a) {
+  P p{};
+  p.B = a->B; p.T = a->T; p.D = a->D; p.N = a->N; p.G = a->G; p.S = a->S; p.softplus = a->softplus;
+  p.cu = a->cu_seqlens;
+  p.x = a->x; p.dt = a->dt; p.z = a->z; p.bm = a->Bm; p.cm = a->Cm;
+  for (int i = 0; i < 2; ++i) {
+    p.xs[i] = a->x_strides[i];
+    p.ds[i] = a->dt_strides[i];
+    p.zs[i] = a->z_strides[i];
+    p.bs[i] = a->b_strides[i];
+    p.cs[i] = a->c_strides[i];
+  }
+  p.A = a->A; p.skip = a->skip; p.bias = a->dt_bias; p.h0 = a->h0;
+  p.y = a->y; p.ht = a->ht; p.states = a->states;
+  const int es = dtype_bytes(a->dtype);
+  const bool ch4 = p.D / p.G % 4 == 0;
+  auto quads = [&](const void* t, const int64_t (&s)[2], bool ok) {
+    return ok && aligned_to(t, 4 * es) && s[0] % 4 == 0 && s[1] % 4 == 0;
+  };
+  p.vx = quads(p.x, p.xs, ch4);
+  p.vd = quads(p.dt, p.ds, ch4);
+  p.vz = quads(p.z, p.zs, ch4);
+  p.vb = quads(p.bm, p.bs, p.N % 4 == 0);
+  p.vc = quads(p.cm, p.cs, p.N % 4 == 0);
+  p.vy = ch4 && aligned_to(p.y, 4 * es);
+  return p;
+}
+
+// calls f with (T, LN, NT, VAR)
+template <typename F>
+int by_shape(const P& p, int dtype, F f) {
+  auto states = [&](auto t, auto var) {
+    if (p.N <= 8) return f(t, std::integral_constant<int, 4>(), std::integral_constant<int, 2>(), var);
+    if (p.N <= 16) return f(t, std::integral_constant<int, 4>(), std::integral_constant<int, 4>(), var);
+    if (p.N <= 32) return f(t, std::integral_constant<int, 8>(), std::integral_constant<int, 4>(), var);
+    return f(t, std::integral_constant<int, 16>(), std::integral_constant<int, 4>(), var);
+  };
+  auto packed = [&](auto t) { return p.cu ? states(t, std::true_type()) : states(t, std::false_type()); };
+  if (dtype == TOPS_F32) return packed(float());
+  if (dtype == TOPS_BF16) return packed(__nv_bfloat16());
+  return packed(__half());
+}
+
+// bump allocator over the caller's workspace (dry run when base == nullptr)
+struct Carve {
+  char* base;
+  size_t used = 0;
+  float* take(size_t count) {
+    used = (used + 255) & ~size_t(255);
+    float* p = base ? reinterpret_cast<float*>(base + used) : nullptr;
+    used += count * sizeof(float);
+    return p;
+  }
+};
+
+// Rows of a segment.  A block walks its rows alone, so without enough blocks the SMs idle; every split costs the
+// exponentials of a first pass.
+inline void split(P& p, int blocks_per_row, int blocks_wanted) {
+  p.seg = std::max(p.T, 1);
+  p.nseg = 1;
+  const int64_t blocks = (int64_t)blocks_per_row * p.B;
+  if (blocks >= blocks_wanted || p.T < 2 * kMinSegment) return;
+  const int want = (int)std::min<int64_t>((2 * blocks_wanted + blocks - 1) / blocks, p.T / kMinSegment);
+  if (want < 2) return;
+  p.seg = ((p.T + want - 1) / want + 31) / 32 * 32;
+  p.nseg = (p.T + p.seg - 1) / p.seg;
+}
+
+inline int lanes_of(int N) { return N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+inline int blocks_of(const P& p, int db) { return (p.D / p.G + db - 1) / db * p.G; }
+
+inline size_t carve_segments(P& p, Carve& c) {
+  if (p.nseg > 1) {
+    p.carry = c.take((size_t)p.B * p.nseg * p.D * p.N);
+    p.sdelta = c.take((size_t)p.B * p.nseg * p.D);
+    p.broken = reinterpret_cast<int*>(c.take(p.nseg));
+  }
+  return c.used;
+}
+
+template <typename F>
+int by_type(int dtype, F f) {
+  if (dtype == TOPS_F32) return f(float());
+  if (dtype == TOPS_BF16) return f(__nv_bfloat16());
+  return f(__half());
+}
+
+inline int empty_states(const P& p, const float* from, float* to, cudaStream_t st) {
+  if (!p.cu || !to) return TOPS_OK;
+  LaunchTimer lt(st, "ssm_scan_empty");
+  const int64_t dn = (int64_t)p.D * p.N;
+  k_scan_empty<<<dim3((unsigned)std::min<int64_t>((dn + 255) / 256, 64), p.S), 256, 0, st>>>(p.S, p.T, dn, p.cu, from, to);
+  TOPS_CUDA_LAUNCH_CHECK("ssm_scan_empty");
+  return TOPS_OK;
+}
+
+}  // namespace ssm
+}  // namespace tops

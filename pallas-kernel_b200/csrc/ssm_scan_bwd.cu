@@ -1,0 +1,496 @@
+// Selective state space scan: the backward (ssm_scan.cuh has the mathematics).
+#include "ssm_scan.cuh"
+
+namespace tops {
+namespace ssm {
+
+constexpr int kBwdThreads = 256;
+template <int LN, int NT>
+constexpr size_t bwd_smem() {
+  return sizeof(float) * CK * ((kBwdThreads / LN) * 6 + 2 * LN * NT + 8 * 2 * LN * NT);
+}
+
+// One segment, tile by tile from its end.  A tile's states are computed again from the saved state before it:
+// its first half once more than its second, so that only 8 rows of states and decays are in registers.
+template <typename T, int LN, int NT, bool VAR>
+__global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
+  constexpr int TS = CK, HALF = 8, DB = kBwdThreads / LN, NP = LN * NT, QC = DB / 4, NH = NT / 2;
+  extern __shared__ __align__(16) float smem[];
+  float2(*su)[DB] = reinterpret_cast<float2(*)[DB]>(smem);                    // delta, delta x
+  float(*sdy)[DB] = reinterpret_cast<float(*)[DB]>(smem + TS * DB * 2);
+  float(*sq)[TS][DB] = reinterpret_cast<float(*)[TS][DB]>(smem + TS * DB * 3);  // sum g B, sum A a g h, sum C h
+  float(*sb)[NP] = reinterpret_cast<float(*)[NP]>(smem + TS * DB * 6);
+  float(*sc)[NP] = reinterpret_cast<float(*)[NP]>(smem + TS * DB * 6 + TS * NP);
+  float(*sr)[TS][2 * NP] = reinterpret_cast<float(*)[TS][2 * NP]>(smem + TS * DB * 6 + TS * NP * 2);  // a warp's dB, dC
+  __shared__ int sflag[TS], sseq[TS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nl = lane % LN, b = blockIdx.y, k = blockIdx.z;
+  const int rep = p.D / p.G, nblk = (rep + DB - 1) / DB, grp = blockIdx.x / nblk, blk = blockIdx.x - grp * nblk;
+  const int c0 = blk * DB, cb = warp * (32 / LN) + lane / LN, n0 = nl * NT;
+  const int64_t dbase = (int64_t)grp * rep + c0;
+  const bool on = c0 + cb < rep;
+  const int64_t d = dbase + cb;
+  const int t_first = k * p.seg, t_end = min(t_first + p.seg, p.T);
+  const int nck = (p.T + CK - 1) / CK;
+
+  float2 A[NH], g[NH], dA[NH];
+  states_load<NT>(p.A + d * p.N, n0, on ? p.N : 0, A);
+#pragma unroll
+  for (int j = 0; j < NH; ++j) {
+    A[j] = mul2(A[j], dup(kLog2e));
+    g[j] = dA[j] = dup(0.f);
+  }
+  if (on) {
+    if (k < p.nseg - 1) states_load<NT>(p.carry + (((int64_t)b * p.nseg + k) * p.D + d) * p.N, n0, p.N, g);
+    else if (!VAR && p.dht) states_load<NT>(p.dht + ((int64_t)b * p.D + d) * p.N, n0, p.N, g);
+  }
+
+  // staging: one quad of channels of one row a thread
+  const int qc = tid % QC, qr = tid / QC;
+  const int valid = min(max(rep - c0 - qc * 4, 0), 4);
+  const int64_t qd = dbase + qc * 4;
+  float bias[4], skip[4], dskip[4], dbias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    bias[i] = p.bias && i < valid ? p.bias[qd + i] : 0.f;
+    skip[i] = p.skip && i < valid ? p.skip[qd + i] : 0.f;
+    dskip[i] = dbias[i] = 0.f;
+  }
+  constexpr int BQ = TS * NP / 4, BN = (BQ + kBwdThreads - 1) / kBwdThreads;
+  Quad<T> xr, dr, zr, gr, br[BN], cr[BN];
+  float2 hr[NH];
+  int flag = 0, seq = 0;
+  auto fetch = [&](int t0) {
+    const int t = t0 + qr;
+    const int v = (qr < TS && t < t_end) ? valid : 0;
+    quad_load<T>(static_cast<const T*>(p.x) + b * p.xs[0] + t * p.xs[1] + qd, p.vx, v, xr);
+    quad_load<T>(static_cast<const T*>(p.dt) + b * p.ds[0] + t * p.ds[1] + qd, p.vd, v, dr);
+    quad_load<T>(static_cast<const T*>(p.dout) + b * p.os[0] + t * p.os[1] + qd, p.vo, v, gr);
+    quad_load<T>(static_cast<const T*>(p.z) + b * p.zs[0] + t * p.zs[1] + qd, p.vz, p.z ? v : 0, zr);
+#pragma unroll
+    for (int j = 0; j < BN; ++j) {
+      const int q = tid + j * kBwdThreads, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4;
+      const int w = (q < BQ && t0 + row < t_end) ? min(max(p.N - n, 0), 4) : 0;
+      quad_load<T>(static_cast<const T*>(p.bm) + b * p.bs[0] + (t0 + row) * p.bs[1] + grp * p.N + n, p.vb, w, br[j]);
+      quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + (t0 + row) * p.cs[1] + grp * p.N + n, p.vc, w, cr[j]);
+    }
+    states_load<NT>(p.states + (((int64_t)b * nck + t0 / CK) * p.D + d) * p.N, n0, on ? p.N : 0, hr);
+    if (VAR && tid < TS) flag = t0 + tid < t_end ? row_flags(p, t0 + tid, seq) : 0;
+  };
+
+  const int last = t_end > t_first ? t_first + (t_end - t_first - 1) / TS * TS : t_first - TS;
+  if (last >= t_first) fetch(last);
+  for (int t0 = last; t0 >= t_first; t0 -= TS) {
+    if (VAR) {
+      if (tid < TS) {
+        sflag[tid] = flag;
+        sseq[tid] = seq;
+      }
+      __syncthreads();
+    }
+    const bool gone = qr >= TS || t0 + qr >= t_end || (VAR && (sflag[qr] & kNone));
+    float xf[4], vf[4], zf[4], gf[4], dl[4], dy[4], zs[4];  // kept for the tile's outputs
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      xf[i] = gone ? 0.f : to_f<T>(xr.v[i]);
+      vf[i] = to_f<T>(dr.v[i]) + bias[i];
+      dl[i] = gone ? 0.f : p.softplus ? softplus(vf[i]) : vf[i];
+      gf[i] = gone ? 0.f : to_f<T>(gr.v[i]);
+      zf[i] = gone ? 0.f : to_f<T>(zr.v[i]);
+      zs[i] = fast_sigmoid(zf[i]);
+      dy[i] = p.z ? gf[i] * zf[i] * zs[i] : gf[i];
+    }
+    if (qr < TS) {
+      *reinterpret_cast<float4*>(&su[qr][qc * 4]) = make_float4(dl[0], dl[0] * xf[0], dl[1], dl[1] * xf[1]);
+      *reinterpret_cast<float4*>(&su[qr][qc * 4 + 2]) = make_float4(dl[2], dl[2] * xf[2], dl[3], dl[3] * xf[3]);
+      *reinterpret_cast<float4*>(&sdy[qr][qc * 4]) = make_float4(dy[0], dy[1], dy[2], dy[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < BN; ++j) {
+      const int q = tid + j * kBwdThreads, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4;
+      if (q < BQ) {
+        const bool none = VAR && (sflag[row] & kNone);
+        float fb[4], fc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          fb[i] = none ? 0.f : to_f<T>(br[j].v[i]);
+          fc[i] = none ? 0.f : to_f<T>(cr[j].v[i]);
+        }
+        *reinterpret_cast<float4*>(&sb[row][n]) = make_float4(fb[0], fb[1], fb[2], fb[3]);
+        *reinterpret_cast<float4*>(&sc[row][n]) = make_float4(fc[0], fc[1], fc[2], fc[3]);
+      }
+    }
+    float2 hs[NH];
+#pragma unroll
+    for (int j = 0; j < NH; ++j) hs[j] = hr[j];
+    __syncthreads();
+    if (t0 > t_first) fetch(t0 - TS);
+
+    // the state before row r (a sequence's first row starts anew)
+    auto enter = [&](int r, float2(&h)[NH]) {
+      if (VAR && (sflag[r] & (kFirst | kNone))) {
+#pragma unroll
+        for (int j = 0; j < NH; ++j) h[j] = dup(0.f);
+        if ((sflag[r] & kFirst) && p.h0 && on) states_load<NT>(p.h0 + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, h);
+      }
+    };
+#pragma unroll 1
+    for (int half = 1; half >= 0; --half) {
+      float2 h[NH];
+#pragma unroll
+      for (int j = 0; j < NH; ++j) h[j] = hs[j];
+      if (half == 1) {
+#pragma unroll
+        for (int r = 0; r < HALF; ++r) {
+          enter(r, h);
+          float2 Bv[NH];
+          pairs_load<NT>(&sb[r][n0], Bv);
+          const float2 q = su[r][cb];
+#pragma unroll
+          for (int j = 0; j < NH; ++j) h[j] = fma2(decay2(q.x, A[j]), h[j], mul2(dup(q.y), Bv[j]));
+        }
+      }
+      const int r0 = half * HALF;
+      float2 a[HALF][NH], hp[HALF + 1][NH];
+#pragma unroll
+      for (int r = 0; r < HALF; ++r) {
+        enter(r0 + r, h);
+        float2 Bv[NH];
+        pairs_load<NT>(&sb[r0 + r][n0], Bv);
+        const float2 q = su[r0 + r][cb];
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+          hp[r][j] = h[j];
+          a[r][j] = decay2(q.x, A[j]);
+          h[j] = fma2(a[r][j], h[j], mul2(dup(q.y), Bv[j]));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NH; ++j) hp[HALF][j] = h[j];
+#pragma unroll
+      for (int r4 = HALF - 4; r4 >= 0; r4 -= 4) {
+        float s1[4], s2[4], s3[4];
+#pragma unroll
+        for (int rr = 3; rr >= 0; --rr) {
+          const int r = r4 + rr;
+          if (VAR && (sflag[r0 + r] & (kLast | kNone))) {
+#pragma unroll
+            for (int j = 0; j < NH; ++j) g[j] = dup(0.f);
+            if ((sflag[r0 + r] & kLast) && p.dht && on)
+              states_load<NT>(p.dht + ((int64_t)sseq[r0 + r] * p.D + d) * p.N, n0, p.N, g);
+          }
+          float2 Bv[NH], Cv[NH], w1 = dup(0.f), w2 = dup(0.f), w3 = dup(0.f);
+          pairs_load<NT>(&sb[r0 + r][n0], Bv);
+          pairs_load<NT>(&sc[r0 + r][n0], Cv);
+          const float2 q = su[r0 + r][cb];
+          const float dyv = sdy[r0 + r][cb];
+          float bc[2 * NT];
+#pragma unroll
+          for (int j = 0; j < NH; ++j) {
+            float2 ht = hp[r + 1][j];
+            if (VAR) ht = fma2(a[r][j], hp[r][j], mul2(dup(q.y), Bv[j]));  // the next row may have started anew
+            g[j] = fma2(Cv[j], dup(dyv), g[j]);
+            w1 = j ? fma2(g[j], Bv[j], w1) : mul2(g[j], Bv[j]);
+            w3 = j ? fma2(Cv[j], ht, w3) : mul2(Cv[j], ht);
+            const float2 vb = mul2(g[j], dup(q.y)), vc = mul2(ht, dup(dyv));
+            bc[2 * j] = vb.x; bc[2 * j + 1] = vb.y;
+            bc[NT + 2 * j] = vc.x; bc[NT + 2 * j + 1] = vc.y;
+            g[j] = mul2(a[r][j], g[j]);
+            const float2 w = mul2(g[j], hp[r][j]);
+            w2 = j ? fma2(A[j], w, w2) : mul2(A[j], w);
+            dA[j] = fma2(dup(q.x), w, dA[j]);
+          }
+          s1[rr] = w1.x + w1.y;
+          s2[rr] = w2.x + w2.y;
+          s3[rr] = w3.x + w3.y;
+          const int at = fold<2 * NT, 32 / LN, LN>(bc, lane);  // over the warp's channels
+          constexpr int KEEP = 2 * NT / (32 / LN) > 1 ? 2 * NT / (32 / LN) : 1;
+#pragma unroll
+          for (int i = 0; i < KEEP; ++i)
+            sr[warp][r0 + r][((at + i) / NT) * NP + n0 + (at + i) % NT] = bc[i];
+          if (VAR && (sflag[r0 + r] & kFirst) && p.dh0 && on)
+            states_store<NT>(p.dh0 + ((int64_t)sseq[r0 + r] * p.D + d) * p.N, n0, p.N, g);
+        }
+        const int o1 = fold<4, LN, 1>(s1, lane);  // over the lanes of a channel
+        fold<4, LN, 1>(s2, lane);
+        fold<4, LN, 1>(s3, lane);
+        sq[0][r0 + r4 + o1][cb] = s1[0];
+        sq[1][r0 + r4 + o1][cb] = s2[0];
+        sq[2][r0 + r4 + o1][cb] = s3[0];
+      }
+    }
+    __syncthreads();
+
+    const int t = t0 + qr;
+    if (qr < TS && t < t_end) {
+      const bool none = VAR && (sflag[qr] & kNone);
+      float odx[4], oddt[4], odz[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float gB = sq[0][qr][qc * 4 + i], aw = sq[1][qr][qc * 4 + i] * kLn2;
+        const float y = fmaf(skip[i], xf[i], sq[2][qr][qc * 4 + i]);
+        odx[i] = none ? 0.f : fmaf(dl[i], gB, skip[i] * dy[i]);
+        float dv = fmaf(xf[i], gB, aw);
+        if (p.softplus) dv *= fast_sigmoid(vf[i]);
+        oddt[i] = none ? 0.f : dv;
+        odz[i] = none ? 0.f : gf[i] * y * zs[i] * fmaf(zf[i], 1.f - zs[i], 1.f);
+        dbias[i] += oddt[i];
+        dskip[i] = fmaf(dy[i], xf[i], dskip[i]);
+      }
+      const int64_t o = ((int64_t)b * p.T + t) * p.D + qd;
+      quad_store<T>(static_cast<T*>(p.dx) + o, p.vg, valid, odx);
+      quad_store<T>(static_cast<T*>(p.ddt) + o, p.vg, valid, oddt);
+      if (p.dz) quad_store<T>(static_cast<T*>(p.dz) + o, p.vg, valid, odz);
+    }
+    float* part = p.pbc + (((int64_t)blockIdx.x * p.B + b) * p.T + t0) * 2 * p.N;
+    for (int i = tid; i < TS * 2 * NP; i += kBwdThreads) {
+      const int row = i / (2 * NP), c = i - row * 2 * NP, n = c % NP;
+      if (t0 + row < t_end && n < p.N) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kBwdThreads / 32; ++w) s += sr[w][row][c];
+        part[(int64_t)row * 2 * p.N + (c / NP) * p.N + n] = s;
+      }
+    }
+    if (VAR) __syncthreads();
+  }
+
+  const int64_t sg = (int64_t)b * p.nseg + k;
+  if (on) {
+    states_store<NT>(p.pa + (sg * p.D + d) * p.N, n0, p.N, dA);
+    if (!VAR && p.dh0 && k == 0) states_store<NT>(p.dh0 + ((int64_t)b * p.D + d) * p.N, n0, p.N, g);
+  }
+  // dD and dbias: the rows' threads of a quad, in a fixed order
+  __syncthreads();
+  float* red = smem;  // [2][TS][DB]
+  if (qr < TS)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      red[qr * DB + qc * 4 + i] = dskip[i];
+      red[(TS + qr) * DB + qc * 4 + i] = dbias[i];
+    }
+  __syncthreads();
+  for (int i = tid; i < 2 * DB; i += kBwdThreads) {
+    const int which = i / DB, c = i - which * DB;
+    if (c0 + c >= rep) continue;
+    float s = 0.f;
+    for (int r = 0; r < (kBwdThreads / QC < TS ? kBwdThreads / QC : TS); ++r) s += red[(which * TS + r) * DB + c];
+    p.pd[(sg * 2 + which) * p.D + dbase + c] = s;
+  }
+}
+
+// The backward's first pass over a segment: the gradient that leaves it with nothing coming in, and the sum of delta.
+template <typename T, int LN, int NT, bool VAR>
+__global__ void __launch_bounds__(128) k_scan_bwd_sum(const P p) {
+  constexpr int TS = 32, DB = 128 / LN, NP = LN * NT, QC = DB / 4, RPP = 128 / QC, QN = RPP >= TS ? 1 : TS / RPP;
+  constexpr int NH = NT / 2, BQ = TS * NP / 4, BN = (BQ + 127) / 128;
+  __shared__ __align__(16) float2 su[TS][DB];  // delta, dy
+  __shared__ __align__(16) float sc[TS][NP];
+  __shared__ int sflag[TS], sseq[TS];
+  const int tid = threadIdx.x, lane = tid & 31, nl = lane % LN, b = blockIdx.y, k = blockIdx.z + 1;  // segment 0 passes nothing on
+  const int rep = p.D / p.G, nblk = (rep + DB - 1) / DB, grp = blockIdx.x / nblk;
+  const int c0 = (blockIdx.x - grp * nblk) * DB, cb = tid / 32 * (32 / LN) + lane / LN, n0 = nl * NT;
+  const int64_t dbase = (int64_t)grp * rep + c0, d = dbase + cb;
+  const bool on = c0 + cb < rep;
+  const int t_first = k * p.seg, t_end = min(t_first + p.seg, p.T);
+  float2 A[NH], g[NH];
+  states_load<NT>(p.A + d * p.N, n0, on ? p.N : 0, A);
+#pragma unroll
+  for (int j = 0; j < NH; ++j) {
+    A[j] = mul2(A[j], dup(kLog2e));
+    g[j] = dup(0.f);
+  }
+  float dsum = 0.f;
+  const int qc = tid % QC, qr = tid / QC;
+  const int valid = min(max(rep - c0 - qc * 4, 0), 4);
+  const int64_t qd = dbase + qc * 4;
+  float bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bias[i] = p.bias && i < valid ? p.bias[qd + i] : 0.f;
+  int broken = 0;
+  const int last = t_first + (t_end - t_first - 1) / TS * TS;
+  for (int t0 = last; t0 >= t_first; t0 -= TS) {
+    int flag = 0, seq = 0;
+    if (VAR) {
+      if (tid < TS) {
+        flag = t0 + tid < t_end ? row_flags(p, t0 + tid, seq) : 0;
+        sflag[tid] = flag;
+        sseq[tid] = seq;
+      }
+      broken |= __syncthreads_or(flag & (kLast | kNone));
+    }
+#pragma unroll
+    for (int j = 0; j < QN; ++j) {
+      const int row = qr + j * RPP, t = t0 + row;
+      if (row >= TS) continue;
+      const bool gone = t >= t_end || (VAR && (sflag[row] & kNone));
+      Quad<T> dr, gr, zr;
+      const int v = gone ? 0 : valid;
+      quad_load<T>(static_cast<const T*>(p.dt) + b * p.ds[0] + t * p.ds[1] + qd, p.vd, v, dr);
+      quad_load<T>(static_cast<const T*>(p.dout) + b * p.os[0] + t * p.os[1] + qd, p.vo, v, gr);
+      quad_load<T>(static_cast<const T*>(p.z) + b * p.zs[0] + t * p.zs[1] + qd, p.vz, p.z ? v : 0, zr);
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float dl = to_f<T>(dr.v[i]) + bias[i];
+        if (p.softplus) dl = softplus(dl);
+        const float z = to_f<T>(zr.v[i]);
+        const float dy = p.z ? to_f<T>(gr.v[i]) * z * fast_sigmoid(z) : to_f<T>(gr.v[i]);
+        f[2 * i] = gone ? 0.f : dl;
+        f[2 * i + 1] = gone ? 0.f : dy;
+      }
+      *reinterpret_cast<float4*>(&su[row][qc * 4]) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(&su[row][qc * 4 + 2]) = make_float4(f[4], f[5], f[6], f[7]);
+    }
+#pragma unroll
+    for (int j = 0; j < BN; ++j) {
+      const int q = tid + j * 128, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4;
+      if (q >= BQ) continue;
+      const bool gone = t0 + row >= t_end || (VAR && (sflag[row] & kNone));
+      Quad<T> cr;
+      quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + (t0 + row) * p.cs[1] + grp * p.N + n, p.vc,
+                   gone ? 0 : min(max(p.N - n, 0), 4), cr);
+      *reinterpret_cast<float4*>(&sc[row][n]) =
+          make_float4(to_f<T>(cr.v[0]), to_f<T>(cr.v[1]), to_f<T>(cr.v[2]), to_f<T>(cr.v[3]));
+    }
+    __syncthreads();
+    for (int r = min(TS, t_end - t0) - 1; r >= 0; --r) {
+      if (VAR && (sflag[r] & (kLast | kNone))) {
+#pragma unroll
+        for (int j = 0; j < NH; ++j) g[j] = dup(0.f);
+        if ((sflag[r] & kLast) && p.dht && on) states_load<NT>(p.dht + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, g);
+      }
+      float2 Cv[NH];
+      pairs_load<NT>(&sc[r][n0], Cv);
+      const float2 q = su[r][cb];
+#pragma unroll
+      for (int j = 0; j < NH; ++j) g[j] = mul2(decay2(q.x, A[j]), fma2(Cv[j], dup(q.y), g[j]));
+      dsum += q.x;
+    }
+    __syncthreads();
+  }
+  if (on) {
+    states_store<NT>(p.carry + (((int64_t)b * p.nseg + k) * p.D + d) * p.N, n0, p.N, g);
+    if (nl == 0) p.sdelta[((int64_t)b * p.nseg + k) * p.D + d] = dsum;
+  }
+  if (VAR && blockIdx.x == 0 && tid == 0) p.broken[k] = broken != 0;
+}
+
+// dB, dC [B, T, G, N] = the parts' sums, in a fixed order
+template <typename T>
+__global__ void k_scan_bc(const P p, T* __restrict__ dB, T* __restrict__ dC) {
+  const int64_t rows = (int64_t)p.B * p.T, per = rows * 2 * p.N;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int grp = blockIdx.y;
+  if (i >= per) return;
+  float s = 0.f;
+  for (int k = 0; k < p.parts; ++k) s += p.pbc[((int64_t)grp * p.parts + k) * per + i];
+  const int64_t row = i / (2 * p.N);
+  const int c = (int)(i - row * 2 * p.N);
+  T* o = c < p.N ? dB : dC;
+  o[(row * p.G + grp) * p.N + (c < p.N ? c : c - p.N)] = from_f<T>(s);
+}
+
+// out[i] = sum over parts of part[k][i], in a fixed order
+__global__ void k_scan_sum(int parts, int64_t n, int64_t stride, const float* __restrict__ part, float* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+  for (int k = 0; k < parts; ++k) s += part[k * stride + i];
+  out[i] = s;
+}
+
+size_t plan_bwd(P& p, void* ws) {
+  p.parts = blocks_of(p, kBwdThreads / lanes_of(p.N)) / p.G;
+  split(p, p.parts * p.G, kBwdBlocks);
+  Carve c{static_cast<char*>(ws)};
+  p.pbc = c.take((size_t)p.G * p.parts * p.B * p.T * 2 * p.N);
+  p.pa = c.take((size_t)p.B * p.nseg * p.D * p.N);
+  p.pd = c.take((size_t)p.B * p.nseg * 2 * p.D);
+  return carve_segments(p, c);
+}
+
+}  // namespace ssm
+}  // namespace tops
+
+using namespace tops;
+using namespace tops::ssm;
+
+extern "C" {
+
+TOPS_API size_t tops_gla_ssm_scan_bwd_workspace_size(const tops_gla_scan_bwd_args* a) {
+  if (a == nullptr || check(&a->f) != TOPS_OK) return 0;
+  P p = params(&a->f);
+  return plan_bwd(p, nullptr);
+}
+
+TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream) {
+  TOPS_CHECK_ARG(a != nullptr, "ssm_scan_bwd: args is NULL");
+  if (int rc = check(&a->f)) return rc;
+  const tops_gla_scan_args& f = a->f;
+  const bool rows = (int64_t)f.B * f.T > 0;
+  TOPS_CHECK_ARG(!rows || (f.x && f.dt && f.Bm && f.Cm && f.A && f.states && a->dout && a->dx && a->ddt && a->dB && a->dC),
+                 "ssm_scan_bwd: x, dt, B, C, A, states, dout and the gradients of x, dt, B and C are required");
+  TOPS_CHECK_ARG(!rows || !f.z || a->dz, "ssm_scan_bwd: z needs dz");
+  P p = params(&f);
+  const size_t need = plan_bwd(p, a->workspace);
+  if (need && (a->workspace == nullptr || a->workspace_bytes < need))
+    return fail(TOPS_ERR_WORKSPACE, "ssm_scan_bwd: workspace smaller than tops_gla_ssm_scan_bwd_workspace_size()");
+  p.dout = a->dout; p.os[0] = a->dout_strides[0]; p.os[1] = a->dout_strides[1];
+  p.dht = a->dht; p.dx = a->dx; p.ddt = a->ddt; p.dz = a->dz; p.dh0 = a->dh0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int rc = empty_states(p, p.dht, p.dh0, st)) return rc;
+  if (p.B > 0) {
+    const int es = dtype_bytes(f.dtype);
+    const bool ch4 = p.D / p.G % 4 == 0;
+    p.vo = ch4 && aligned_to(p.dout, 4 * es) && p.os[0] % 4 == 0 && p.os[1] % 4 == 0;
+    p.vg = ch4 && aligned_to(p.dx, 4 * es) && aligned_to(p.ddt, 4 * es) && aligned_to(p.dz, 4 * es);
+    if (p.nseg > 1) {
+      LaunchTimer lt(st, "ssm_scan_bwd_sum");
+      by_shape(p, f.dtype, [&](auto t, auto ln, auto nt, auto var) {
+        constexpr int LN = decltype(ln)::value;
+        k_scan_bwd_sum<decltype(t), LN, decltype(nt)::value, decltype(var)::value>
+            <<<dim3(blocks_of(p, 128 / LN), p.B, p.nseg - 1), 128, 0, st>>>(p);
+        return 0;
+      });
+      TOPS_CUDA_LAUNCH_CHECK("ssm_scan_bwd_sum");
+      k_scan_chain<true><<<dim3((unsigned)(((int64_t)p.D * p.N + 127) / 128), p.B), 128, 0, st>>>(p);
+      TOPS_CUDA_LAUNCH_CHECK("ssm_scan_chain");
+    }
+    LaunchTimer lt(st, "ssm_scan_bwd");
+    const int rc = by_shape(p, f.dtype, [&](auto t, auto ln, auto nt, auto var) {
+      constexpr int LN = decltype(ln)::value, NT = decltype(nt)::value;
+      auto kernel = k_scan_bwd<decltype(t), LN, NT, decltype(var)::value>;
+      constexpr size_t bytes = bwd_smem<LN, NT>();
+      if (bytes > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return cuda_status(e, "ssm_scan_bwd");
+      }
+      kernel<<<dim3(p.parts * p.G, p.B, p.nseg), kBwdThreads, bytes, st>>>(p);
+      return 0;
+    });
+    if (rc) return rc;
+    TOPS_CUDA_LAUNCH_CHECK("ssm_scan_bwd");
+  }
+  if (rows) {
+    LaunchTimer lt(st, "ssm_scan_bc");
+    const int64_t per = (int64_t)p.B * p.T * 2 * p.N;
+    by_type(f.dtype, [&](auto t) {
+      using T = decltype(t);
+      k_scan_bc<T><<<dim3((unsigned)((per + 255) / 256), p.G), 256, 0, st>>>(p, static_cast<T*>(a->dB), static_cast<T*>(a->dC));
+      return 0;
+    });
+    TOPS_CUDA_LAUNCH_CHECK("ssm_scan_bc");
+  }
+  const struct { int64_t n, stride; const float* part; float* out; } sums[] = {
+      {(int64_t)p.D * p.N, (int64_t)p.D * p.N, p.pa, a->dA}, {p.D, 2 * (int64_t)p.D, p.pd, a->dskip},
+      {p.D, 2 * (int64_t)p.D, p.pd + p.D, a->ddt_bias}};
+  for (const auto& s : sums) {
+    if (!s.out) continue;
+    LaunchTimer lt(st, "ssm_scan_sum");
+    k_scan_sum<<<(unsigned)((s.n + 255) / 256), 256, 0, st>>>(p.B * p.nseg, s.n, s.stride, s.part, s.out);
+    TOPS_CUDA_LAUNCH_CHECK("ssm_scan_sum");
+  }
+  return TOPS_OK;
+}
+
+}  // extern "C"
