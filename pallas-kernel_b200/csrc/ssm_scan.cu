@@ -99,10 +99,10 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
           float f[4];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float dl = to_f<T>(dr[j].v[i + e]) + bias[i + e];
+            float dl = dr[j].get(i + e) + bias[i + e];
             if (p.softplus) dl = softplus(dl);
             f[2 * e] = gone ? 0.f : dl;
-            f[2 * e + 1] = gone ? 0.f : dl * to_f<T>(xr[j].v[i + e]);
+            f[2 * e + 1] = gone ? 0.f : dl * xr[j].get(i + e);
           }
           *reinterpret_cast<float4*>(&su[row][qc * 4 + i]) = make_float4(f[0], f[1], f[2], f[3]);
         }
@@ -116,8 +116,8 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
         float fb[4], fc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          fb[i] = gone ? 0.f : to_f<T>(br[j].v[i]);
-          fc[i] = SUM || gone ? 0.f : to_f<T>(cr[j].v[i]);
+          fb[i] = gone ? 0.f : br[j].get(i);
+          fc[i] = SUM || gone ? 0.f : cr[j].get(i);
         }
         *reinterpret_cast<float4*>(&sb[row][n]) = make_float4(fb[0], fb[1], fb[2], fb[3]);
         if (!SUM) *reinterpret_cast<float4*>(&sc[row][n]) = make_float4(fc[0], fc[1], fc[2], fc[3]);
@@ -197,9 +197,9 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
           const bool gone = VAR && (sflag[row] & kNone);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            o[i] = fmaf(skip[i], to_f<T>(xc[j].v[i]), o[i]);
+            o[i] = fmaf(skip[i], xc[j].get(i), o[i]);
             if (p.z) {
-              const float z = to_f<T>(zc[j].v[i]);
+              const float z = zc[j].get(i);
               o[i] *= z * fast_sigmoid(z);
             }
             if (gone) o[i] = 0.f;

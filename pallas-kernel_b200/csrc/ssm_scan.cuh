@@ -115,21 +115,43 @@ __device__ __forceinline__ int fold(float (&v)[V], int lane) {
   return off;
 }
 
-// four elements of T (those at `valid` and beyond are zero)
+// Four elements of T as they lie in memory (those at `valid` and beyond are zero).  They are taken apart where they
+// are used, a tile later: a load's registers may not be touched before.
 template <typename T>
 struct Quad {
-  T v[4];
+  uint32_t w[sizeof(T)];  // 4 sizeof(T) bytes
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint16_t h = (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
+      if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(h));
+      else return __uint_as_float((uint32_t)h << 16);
+    }
+  }
 };
 template <typename T>
 __device__ __forceinline__ void quad_load(const T* p, bool vec, int valid, Quad<T>& q) {
-  if (vec && valid >= 4) {
-    alignas(16) T raw[4];
-    Vx<T, 4>::load_raw(p, raw);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = raw[i];
+  for (int i = 0; i < (int)sizeof(T); ++i) q.w[i] = 0;
+  if (vec) {
+    if (valid >= 4) {
+      if constexpr (sizeof(T) == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        q.w[0] = v.x; q.w[1] = v.y; q.w[2] = v.z; q.w[3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        q.w[0] = v.x; q.w[1] = v.y;
+      }
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = i < valid ? p[i] : from_f<T>(0.f);
+    for (int i = 0; i < 4; ++i) {
+      if (i < valid) {
+        if constexpr (sizeof(T) == 4) q.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+        else q.w[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+      }
+    }
   }
 }
 template <typename T>

@@ -91,11 +91,11 @@ __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
     float xf[4], vf[4], zf[4], gf[4], dl[4], dy[4], zs[4];  // kept for the tile's outputs
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      xf[i] = gone ? 0.f : to_f<T>(xr.v[i]);
-      vf[i] = to_f<T>(dr.v[i]) + bias[i];
+      xf[i] = gone ? 0.f : xr.get(i);
+      vf[i] = dr.get(i) + bias[i];
       dl[i] = gone ? 0.f : p.softplus ? softplus(vf[i]) : vf[i];
-      gf[i] = gone ? 0.f : to_f<T>(gr.v[i]);
-      zf[i] = gone ? 0.f : to_f<T>(zr.v[i]);
+      gf[i] = gone ? 0.f : gr.get(i);
+      zf[i] = gone ? 0.f : zr.get(i);
       zs[i] = fast_sigmoid(zf[i]);
       dy[i] = p.z ? gf[i] * zf[i] * zs[i] : gf[i];
     }
@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
         float fb[4], fc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          fb[i] = none ? 0.f : to_f<T>(br[j].v[i]);
-          fc[i] = none ? 0.f : to_f<T>(cr[j].v[i]);
+          fb[i] = none ? 0.f : br[j].get(i);
+          fc[i] = none ? 0.f : cr[j].get(i);
         }
         *reinterpret_cast<float4*>(&sb[row][n]) = make_float4(fb[0], fb[1], fb[2], fb[3]);
         *reinterpret_cast<float4*>(&sc[row][n]) = make_float4(fc[0], fc[1], fc[2], fc[3]);
@@ -331,10 +331,10 @@ __global__ void __launch_bounds__(128) k_scan_bwd_sum(const P p) {
       float f[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float dl = to_f<T>(dr.v[i]) + bias[i];
+        float dl = dr.get(i) + bias[i];
         if (p.softplus) dl = softplus(dl);
-        const float z = to_f<T>(zr.v[i]);
-        const float dy = p.z ? to_f<T>(gr.v[i]) * z * fast_sigmoid(z) : to_f<T>(gr.v[i]);
+        const float z = zr.get(i);
+        const float dy = p.z ? gr.get(i) * z * fast_sigmoid(z) : gr.get(i);
         f[2 * i] = gone ? 0.f : dl;
         f[2 * i + 1] = gone ? 0.f : dy;
       }
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(128) k_scan_bwd_sum(const P p) {
       quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + (t0 + row) * p.cs[1] + grp * p.N + n, p.vc,
                    gone ? 0 : min(max(p.N - n, 0), 4), cr);
       *reinterpret_cast<float4*>(&sc[row][n]) =
-          make_float4(to_f<T>(cr.v[0]), to_f<T>(cr.v[1]), to_f<T>(cr.v[2]), to_f<T>(cr.v[3]));
+          make_float4(cr.get(0), cr.get(1), cr.get(2), cr.get(3));
     }
     __syncthreads();
     for (int r = min(TS, t_end - t0) - 1; r >= 0; --r) {
