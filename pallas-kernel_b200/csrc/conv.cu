@@ -15,7 +15,7 @@ namespace conv {
 
 struct P {
   int B, T, D, N;  // N sequences
-  int act, wdtype;
+  int act, wdtype, wvec;  // wvec: the weights of V channels start on a vector
   const int32_t* cu;
   int64_t xb, xt;  // strides of x in elements (batch, row)
   const void* x;
@@ -39,6 +39,36 @@ __device__ __forceinline__ float act_grad(float p, int act) {
   if (!act) return 1.f;
   const float s = fast_sigmoid(p);
   return s * fmaf(p, 1.f - s, 1.f);
+}
+
+// weights [V][W] and biases of V channels from d0: V W elements in a row
+template <typename T, int V, int W>
+__device__ __forceinline__ void load_params(const P& p, int d0, float (&w)[W][V], float (&bias)[V]) {
+  float flat[W][V];  // W vectors of V elements
+  if (p.wdtype == TOPS_F32 && sizeof(T) != 4) {
+    const float* wp = static_cast<const float*>(p.w) + (int64_t)d0 * W;
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) flat[j][i] = wp[j * V + i];
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias[i] = p.b ? static_cast<const float*>(p.b)[d0 + i] : 0.f;
+  } else {
+    const T* wp = static_cast<const T*>(p.w) + (int64_t)d0 * W;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      if (p.wvec) Vx<T, V>::load(wp + j * V, flat[j]);
+      else
+#pragma unroll
+        for (int i = 0; i < V; ++i) flat[j][i] = to_f<T>(wp[j * V + i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias[i] = p.b ? to_f<T>(static_cast<const T*>(p.b)[d0 + i]) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j][i] = flat[(i * W + j) / V][(i * W + j) % V];
 }
 
 // the sequence of row t of batch row b: [s, e) and its number (-1: none)
@@ -84,6 +114,7 @@ __device__ void final_state(const P& p, int n, int d0) {
 
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
+  constexpr int R = 4;
   const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
   const int64_t unit = id / p.dv;
   const int d0 = (int)(id - unit * p.dv) * V;
@@ -97,19 +128,15 @@ __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
   const int t0 = (int)(unit - (int64_t)b * p.strips) * p.strip;
   const int t1 = min(t0 + p.strip, p.T);
   float w[W][V], bias[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[j][i] = load_param(p.w, p.wdtype, (int64_t)(d0 + i) * W + j);
-    bias[i] = p.b ? load_param(p.b, p.wdtype, d0 + i) : 0.f;
-  }
+  load_params<T, V, W>(p, d0, w, bias);
   const T* x = static_cast<const T*>(p.x) + b * p.xb + d0;
   T* y = static_cast<T*>(p.y) + (int64_t)b * p.T * p.D + d0;
   SeqAt q = seq_of(p, b, t0);
   float win[W][V];  // rows t - W + 1 .. t
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) row_or_state<T, V, W>(p, b, q, t0 - (W - 1) + j, d0, win[j + 1]);
-  for (int t = t0; t < t1; ++t) {
+  // one row, at any place of its sequence
+  auto row = [&](int t) {
     if (t >= q.e || q.n < 0) {
       q = seq_of(p, b, t);
       if (q.n < 0) {
@@ -117,7 +144,7 @@ __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) zero[i] = 0.f;
         Vx<T, V>::store(y + (int64_t)t * p.D, zero);
-        continue;
+        return;
       }
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) row_or_state<T, V, W>(p, b, q, t - (W - 1) + j, d0, win[j + 1]);
@@ -136,21 +163,57 @@ __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
       out[i] = act_fwd(a, p.act);
     }
     Vx<T, V>::store(y + (int64_t)t * p.D, out);
+  };
+  // R rows inside one sequence: their loads are issued R rows ahead of their use
+  Raw<T, V> next[R];
+  int have = -1;  // first row in `next`
+  for (int t = t0; t < t1;) {
+    if (t + R > t1 || t + R > q.e || q.n < 0) {
+      row(t++);
+      continue;
+    }
+    if (have != t)
+#pragma unroll
+      for (int r = 0; r < R; ++r) next[r].load(x + (t + r) * p.xt);
+    Raw<T, V> cur[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) cur[r] = next[r];
+    if (t + 2 * R <= t1) {
+      have = t + R;
+#pragma unroll
+      for (int r = 0; r < R; ++r) next[r].load(x + (t + R + r) * p.xt);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
+      cur[r].get(win[W - 1]);
+      float out[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float a = bias[i];
+#pragma unroll
+        for (int j = 0; j < W; ++j) a = fmaf(w[j][i], win[j][i], a);
+        out[i] = act_fwd(a, p.act);
+      }
+      Vx<T, V>::store(y + (int64_t)(t + r) * p.D, out);
+    }
+    t += R;
   }
 }
 
-// dp of row t of sequence q (channels d0..) from its window
-template <typename T, int V, int W>
+// dp of a row from its window; dp holds the row's dy
+template <int V, int W>
 __device__ __forceinline__ void dp_of(const P& p, const float (&w)[W][V], const float (&bias)[V],
-                                      const float (&win)[W][V], int b, int t, int d0, float (&dp)[V]) {
-  float g[V];
-  Vx<T, V>::load(static_cast<const T*>(p.dy) + b * p.gb + t * p.gt + d0, g);
+                                      const float (&win)[W][V], float (&dp)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float a = bias[i];
 #pragma unroll
     for (int j = 0; j < W; ++j) a = fmaf(w[j][i], win[j][i], a);
-    dp[i] = g[i] * act_grad(a, p.act);
+    dp[i] *= act_grad(a, p.act);
   }
 }
 
@@ -178,7 +241,8 @@ __device__ void state_grad(const P& p, const float (&w)[W][V], const float (&bia
       float win[W][V], dp[V];
 #pragma unroll
       for (int j = 0; j < W; ++j) row_or_state<T, V, W>(p, b, q, q.s + r - (W - 1) + j, d0, win[j]);
-      dp_of<T, V, W>(p, w, bias, win, b, q.s + r, d0, dp);
+      Vx<T, V>::load(static_cast<const T*>(p.dy) + b * p.gb + (q.s + r) * p.gt + d0, dp);
+      dp_of<V, W>(p, w, bias, win, dp);
 #pragma unroll
       for (int c = r; c < W - 1; ++c)
 #pragma unroll
@@ -204,18 +268,14 @@ __device__ void state_grad(const P& p, const float (&w)[W][V], const float (&bia
 // strip, whose rows alone go into dw and db).
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
+  constexpr int R = 4;
   const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
   const int64_t unit = id / p.dv;
   const int d0 = (int)(id - unit * p.dv) * V;
   const int64_t nstrips = (int64_t)p.B * p.strips;
   if (unit >= nstrips && (p.dstate == nullptr || unit - nstrips >= p.N)) return;
   float w[W][V], bias[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[j][i] = load_param(p.w, p.wdtype, (int64_t)(d0 + i) * W + j);
-    bias[i] = p.b ? load_param(p.b, p.wdtype, d0 + i) : 0.f;
-  }
+  load_params<T, V, W>(p, d0, w, bias);
   if (unit >= nstrips) {
     state_grad<T, V, W>(p, w, bias, (int)(unit - nstrips), d0);
     return;
@@ -224,6 +284,7 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
   const int t0 = (int)(unit - (int64_t)b * p.strips) * p.strip;
   const int t1 = min(t0 + p.strip, p.T);
   const T* x = static_cast<const T*>(p.x) + b * p.xb + d0;
+  const T* dy = static_cast<const T*>(p.dy) + b * p.gb + d0;
   T* dx = static_cast<T*>(p.dx) + (int64_t)b * p.T * p.D + d0;
   SeqAt q = seq_of(p, b, t0);
   float win[W][V], acc[W][V], dw[W][V], db[V];  // acc[k]: dx of row t - k so far
@@ -235,8 +296,8 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
     for (int i = 0; i < V; ++i) acc[j][i] = dw[j][i] = 0.f;
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) row_or_state<T, V, W>(p, b, q, t0 - (W - 1) + j, d0, win[j + 1]);
-  const int last = t1 + W - 1;  // rows past T or the sequence add nothing
-  for (int t = t0; t < last; ++t) {
+  // one row, at any place of its sequence (rows past T or the sequence add nothing)
+  auto row = [&](int t) {
     if (t < p.T && (t >= q.e || q.n < 0)) {
       q = seq_of(p, b, t);
 #pragma unroll
@@ -253,9 +314,10 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[0][i] = 0.f;
     if (t < p.T && q.n >= 0) {
-      Vx<T, V>::load(x + t * p.xt, win[W - 1]);
       float dp[V];
-      dp_of<T, V, W>(p, w, bias, win, b, t, d0, dp);
+      Vx<T, V>::load(x + t * p.xt, win[W - 1]);
+      Vx<T, V>::load(dy + t * p.gt, dp);
+      dp_of<V, W>(p, w, bias, win, dp);
 #pragma unroll
       for (int k = 0; k < W; ++k)
         if (t - k >= q.s)
@@ -276,6 +338,62 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
       }
     }
     if (t - (W - 1) >= t0) Vx<T, V>::store(dx + (int64_t)(t - (W - 1)) * p.D, acc[W - 1]);
+  };
+  // R rows inside one sequence, W - 1 rows or more from either end of it and inside the strip: their loads are
+  // issued R rows ahead of their use
+  Raw<T, V> nx[R], ng[R];
+  int have = -1;
+  for (int t = t0; t < t1 + W - 1;) {
+    if (q.n < 0 || t < max(q.s, t0) + W - 1 || t + R > min(t1, q.e - (W - 1))) {
+      row(t++);
+      continue;
+    }
+    if (have != t)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        nx[r].load(x + (t + r) * p.xt);
+        ng[r].load(dy + (t + r) * p.gt);
+      }
+    Raw<T, V> cx[R], cg[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      cx[r] = nx[r];
+      cg[r] = ng[r];
+    }
+    if (t + 2 * R <= t1) {
+      have = t + R;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        nx[r].load(x + (t + R + r) * p.xt);
+        ng[r].load(dy + (t + R + r) * p.gt);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
+#pragma unroll
+      for (int j = W - 1; j > 0; --j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[j][i] = acc[j - 1][i];
+      float dp[V];
+      cx[r].get(win[W - 1]);
+      cg[r].get(dp);
+      dp_of<V, W>(p, w, bias, win, dp);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        acc[0][i] = w[W - 1][i] * dp[i];
+#pragma unroll
+        for (int k = 1; k < W; ++k) acc[k][i] = fmaf(w[W - 1 - k][i], dp[i], acc[k][i]);
+        db[i] += dp[i];
+#pragma unroll
+        for (int j = 0; j < W; ++j) dw[j][i] = fmaf(dp[i], win[j][i], dw[j][i]);
+      }
+      Vx<T, V>::store(dx + (int64_t)(t + r - (W - 1)) * p.D, acc[W - 1]);
+    }
+    t += R;
   }
   if (p.part != nullptr) {
     float* o = p.part + unit * (W + 1) * p.D + d0;
@@ -328,13 +446,14 @@ __global__ void __launch_bounds__(128) k_conv_step(const P p) {
 #pragma unroll
     for (int i = 0; i < V; ++i) st[j * V + i] = v[i];
   }
+  float w[W][V], bias[V];
+  load_params<T, V, W>(p, d0, w, bias);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    float a = p.b ? load_param(p.b, p.wdtype, d0 + i) : 0.f;
+    float a = bias[i];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j)
-      a = fmaf(load_param(p.w, p.wdtype, (int64_t)(d0 + i) * W + j), st[i * (W - 1) + j], a);
-    a = fmaf(load_param(p.w, p.wdtype, (int64_t)(d0 + i) * W + W - 1), x[i], a);
+    for (int j = 0; j < W - 1; ++j) a = fmaf(w[j][i], st[i * (W - 1) + j], a);
+    a = fmaf(w[W - 1][i], x[i], a);
     out[i] = act_fwd(a, p.act);
   }
   Vx<T, V>::store(static_cast<T*>(p.y) + b * p.D + d0, out);
@@ -358,8 +477,8 @@ int by_width(int W, F f) {
   return f(std::integral_constant<int, 4>());
 }
 
-// calls f with (T, V, W); V is 16 bytes of channels where every base and stride allows it, else 1
-template <typename F>
+// calls f with (T, V, W); V is V16 channels (four in fp32) where every base and stride allows 16-byte accesses, else 1
+template <int V16, typename F>
 int by_type(int dtype, bool wide, int W, F f) {
   return by_width(W, [&](auto w) {
     constexpr int WW = decltype(w)::value;
@@ -367,9 +486,9 @@ int by_type(int dtype, bool wide, int W, F f) {
       return wide ? f(float(), std::integral_constant<int, 4>(), std::integral_constant<int, WW>())
                   : f(float(), std::integral_constant<int, 1>(), std::integral_constant<int, WW>());
     if (dtype == TOPS_BF16)
-      return wide ? f(__nv_bfloat16(), std::integral_constant<int, 8>(), std::integral_constant<int, WW>())
+      return wide ? f(__nv_bfloat16(), std::integral_constant<int, V16>(), std::integral_constant<int, WW>())
                   : f(__nv_bfloat16(), std::integral_constant<int, 1>(), std::integral_constant<int, WW>());
-    return wide ? f(__half(), std::integral_constant<int, 8>(), std::integral_constant<int, WW>())
+    return wide ? f(__half(), std::integral_constant<int, V16>(), std::integral_constant<int, WW>())
                 : f(__half(), std::integral_constant<int, 1>(), std::integral_constant<int, WW>());
   });
 }
@@ -400,6 +519,7 @@ P params(const tops_gla_conv_args* a) {
   P p{};
   p.B = a->B; p.T = a->T; p.D = a->D; p.N = a->N;
   p.act = a->activation; p.wdtype = a->w_dtype;
+  p.wvec = aligned_to(a->w, 16);
   p.cu = a->cu_seqlens;
   p.xb = a->x_stride_b; p.xt = a->x_stride_t;
   p.x = a->x; p.w = a->w; p.b = a->bias; p.state = a->initial_state;
@@ -435,7 +555,7 @@ TOPS_API int tops_gla_causal_conv_fwd(const tops_gla_conv_args* a, void* stream)
   const bool wide = wide_ok(a) && aligned_to(a->y, 16);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchTimer lt(st, "causal_conv_fwd");
-  by_type(a->dtype, wide, a->W, [&](auto t, auto v, auto w) {
+  by_type<8>(a->dtype, wide, a->W, [&](auto t, auto v, auto w) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value, W = decltype(w)::value;
     P p = params(a);
@@ -451,7 +571,7 @@ TOPS_API int tops_gla_causal_conv_fwd(const tops_gla_conv_args* a, void* stream)
 TOPS_API size_t tops_gla_causal_conv_bwd_workspace_size(const tops_gla_conv_bwd_args* a) {
   if (a == nullptr || check(&a->f) != TOPS_OK || (!a->dw && !a->dbias)) return 0;
   size_t most = 0;  // of the two layouts (the alignment of the pointers decides between them)
-  for (int v : {1, 16 / dtype_bytes(a->f.dtype)}) {
+  for (int v : {1, 4}) {
     if (a->f.D % v) continue;
     P p = params(&a->f);
     split(p, v, kBwdThreads, 256);
@@ -477,7 +597,7 @@ TOPS_API int tops_gla_causal_conv_bwd(const tops_gla_conv_bwd_args* a, void* str
   int64_t strips = 0;
   if (rows || a->dstate) {
     LaunchTimer lt(st, "causal_conv_bwd");
-    by_type(f.dtype, wide, f.W, [&](auto t, auto v, auto w) {
+    by_type<4>(f.dtype, wide, f.W, [&](auto t, auto v, auto w) {
       using T = decltype(t);
       constexpr int V = decltype(v)::value, W = decltype(w)::value;
       P p = params(&f);
@@ -512,7 +632,7 @@ TOPS_API int tops_gla_causal_conv_step(const tops_gla_conv_args* a, void* stream
                     aligned_to(a->final_state, 16);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchTimer lt(st, "causal_conv_step");
-  by_type(a->dtype, wide, a->W, [&](auto t, auto v, auto w) {
+  by_type<8>(a->dtype, wide, a->W, [&](auto t, auto v, auto w) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value, W = decltype(w)::value;
     P p = params(a);

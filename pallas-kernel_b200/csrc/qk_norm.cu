@@ -20,6 +20,7 @@ struct P {
   int64_t tokens;
   int T, H, HK, K, R, pairs, wdtype, pos64, table;
   int lanes, hg, nhg;  // lanes of a row, heads of a unit, units of a token
+  int wvec;            // the weights start on a vector
   float eps;
   const void *q, *k, *qw, *kw;
   int64_t qs[3], ks[3];  // strides (batch, row, head) of q and k in elements
@@ -33,11 +34,6 @@ struct P {
   void *dq, *dk;
   float* part;  // [blocks][2][K]
 };
-
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 
 // What a lane needs of one vector (elements e0 .. e0 + V): where the partners are and the angle's
 // cosine and signed sine (y_i = n_i c_i + n_partner s_i).
@@ -85,85 +81,210 @@ __device__ __forceinline__ Rot<V> rotation(const P& p, int e0, int64_t pos, floa
   return r;
 }
 
-template <int V>
-__device__ __forceinline__ void weights(const void* w, int dtype, int e0, bool on, float (&r)[V]) {
+// V weights from element e0 (ones without weights); e0 is a multiple of V
+template <typename T, int V>
+__device__ __forceinline__ void weights(const void* w, const P& p, int e0, float (&r)[V]) {
+  if (w == nullptr || e0 >= p.K) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) r[i] = on && w ? load_param(w, dtype, e0 + i) : 1.f;
+    for (int i = 0; i < V; ++i) r[i] = 1.f;
+  } else if (p.wvec && p.wdtype == TOPS_F32) {
+    Vx<float, V>::load(static_cast<const float*>(w) + e0, r);
+  } else if (p.wvec) {
+    Vx<T, V>::load(static_cast<const T*>(w) + e0, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = load_param(w, p.wdtype, e0 + i);
+  }
+}
+
+// The heads h0 .. h1 of q (or of k) of one token, HB at a time: their loads are issued before the first sum.
+// Every lane of a warp takes the same turns, since the sums are full-warp exchanges; `live` says whose rows exist.
+template <typename T, int V, int J, int HB>
+__device__ __forceinline__ void heads_fwd(const P& p, const T* x, int64_t hs, T* y, const void* weight, int h0, int h1,
+                                          int turns, bool live, int l, const Rot<V> (&rot)[J]) {
+  float w[J][V], pw[J][V];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    weights<T, V>(weight, p, (l + j * p.lanes) * V, w[j]);
+    weights<T, V>(weight, p, rot[j].p0, pw[j]);
+  }
+  for (int i = 0; i < turns; i += HB) {
+    Raw<T, V> own[HB][J], par[HB][J];
+#pragma unroll
+    for (int u = 0; u < HB; ++u)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int e0 = (l + j * p.lanes) * V;
+        if (live && h0 + i + u < h1 && e0 < p.K) {
+          own[u][j].load(x + (h0 + i + u) * hs + e0);
+          if (rot[j].on && !(p.pairs && V > 1)) par[u][j].load(x + (h0 + i + u) * hs + rot[j].p0);
+        }
+      }
+    float ss[HB];
+#pragma unroll
+    for (int u = 0; u < HB; ++u) {
+      ss[u] = 0.f;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        if (live && h0 + i + u < h1 && (l + j * p.lanes) * V < p.K) {
+          float v[V];
+          own[u][j].get(v);
+#pragma unroll
+          for (int c = 0; c < V; ++c) ss[u] = fmaf(v[c], v[c], ss[u]);
+        }
+      }
+    }
+    for (int o = p.lanes >> 1; o > 0; o >>= 1)
+#pragma unroll
+      for (int u = 0; u < HB; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
+#pragma unroll
+    for (int u = 0; u < HB; ++u) {
+      const float s = rsqrtf(ss[u] / (float)p.K + p.eps);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int e0 = (l + j * p.lanes) * V;
+        if (live && h0 + i + u < h1 && e0 < p.K) {
+          float out[V];
+          own[u][j].get(out);
+#pragma unroll
+          for (int c = 0; c < V; ++c) out[c] *= s * w[j][c];
+          if (rot[j].on) {
+            float o[V];
+            if (p.pairs && V > 1) {
+#pragma unroll
+              for (int c = 0; c < V; ++c) o[c] = out[c ^ (V > 1 ? 1 : 0)];
+            } else {
+              par[u][j].get(o);
+#pragma unroll
+              for (int c = 0; c < V; ++c) o[c] *= s * pw[j][c];
+            }
+#pragma unroll
+            for (int c = 0; c < V; ++c) out[c] = fmaf(out[c], rot[j].c[c], o[c] * rot[j].s[c]);
+          }
+          Vx<T, V>::store(y + (h0 + i + u) * p.K + e0, out);
+        }
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ int64_t position(const P& p, int b, int t) {
+  if (!p.R || !p.pos) return t;
+  return p.pos64 ? static_cast<const int64_t*>(p.pos)[b * p.pb + t] : static_cast<const int32_t*>(p.pos)[b * p.pb + t];
 }
 
 template <typename T, int V, int J>
 __global__ void __launch_bounds__(256) k_qk_fwd(const P p) {
+  constexpr int HB = J == 1 ? 4 : 1;
   const int lane = threadIdx.x & 31, l = lane & (p.lanes - 1);
   const int rpw = 32 / p.lanes;
   const int64_t unit = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * rpw + lane / p.lanes;
   const bool live = unit < p.tokens * p.nhg;
   const int64_t tok = live ? unit / p.nhg : 0;
-  const int h0 = live ? (int)(unit - tok * p.nhg) * p.hg : 0;
+  const int h0 = live ? (int)(unit - tok * p.nhg) * p.hg : 0, h1 = h0 + p.hg;
   const int b = (int)(tok / p.T), t = (int)(tok - (int64_t)b * p.T);
-  int64_t pos = t;
-  if (p.R && p.pos)
-    pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[b * p.pb + t] : static_cast<const int32_t*>(p.pos)[b * p.pb + t];
+  const int64_t pos = position(p, b, t);
   Rot<V> rot[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int e0 = (l + j * p.lanes) * V;
     rot[j] = rotation<V>(p, e0 < p.K ? e0 : p.K, pos, 1.f);
   }
-  const int heads = p.H + p.HK;
-  for (int i = 0; i < p.hg; ++i) {  // every lane of the warp takes every turn (the sums are full-warp shuffles)
-    const int h = h0 + i;
-    const bool on = live && h < heads, isq = h < p.H;
-    const int hh = isq ? h : h - p.H;
-    const T* x = isq ? static_cast<const T*>(p.q) + b * p.qs[0] + t * p.qs[1] + hh * p.qs[2]
-                     : static_cast<const T*>(p.k) + b * p.ks[0] + t * p.ks[1] + hh * p.ks[2];
-    float v[J][V], ss = 0.f;
+  // units of a warp may lie on both sides of the border between q and k: each side's turns are the warp's most
+  const int q1 = min(h1, p.H), k0 = max(h0, p.H) - p.H, k1 = min(h1, p.H + p.HK) - p.H;
+  const int qn = __reduce_max_sync(0xffffffffu, live ? max(q1 - h0, 0) : 0);
+  const int kn = __reduce_max_sync(0xffffffffu, live ? max(k1 - k0, 0) : 0);
+  if (qn > 0)
+    heads_fwd<T, V, J, HB>(p, static_cast<const T*>(p.q) + b * p.qs[0] + t * p.qs[1], p.qs[2],
+                           static_cast<T*>(p.yq) + tok * p.H * p.K, p.qw, h0, q1, qn, live, l, rot);
+  if (kn > 0)
+    heads_fwd<T, V, J, HB>(p, static_cast<const T*>(p.k) + b * p.ks[0] + t * p.ks[1], p.ks[2],
+                           static_cast<T*>(p.yk) + tok * p.HK * p.K, p.kw, k0, k1, kn, live, l, rot);
+}
+
+// As heads_fwd: both sums of a row (x^2 and e x) come from the same loads; the rows' dw terms are kept.
+template <typename T, int V, int J, int HB>
+__device__ __forceinline__ void heads_bwd(const P& p, const T* x, int64_t hs, const T* dy, int64_t gs, T* dx,
+                                          const void* weight, int h0, int h1, int turns, bool live, int l,
+                                          const Rot<V> (&rot)[J], float (&dw)[J][V]) {
+  float w[J][V];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int e0 = (l + j * p.lanes) * V;
-      if (on && e0 < p.K) {
-        Vx<T, V>::load(x + e0, v[j]);
+  for (int j = 0; j < J; ++j) weights<T, V>(weight, p, (l + j * p.lanes) * V, w[j]);
+  for (int i = 0; i < turns; i += HB) {
+    Raw<T, V> xr[HB][J], gr[HB][J], pr[HB][J];
 #pragma unroll
-        for (int c = 0; c < V; ++c) ss = fmaf(v[j][c], v[j][c], ss);
+    for (int u = 0; u < HB; ++u)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int e0 = (l + j * p.lanes) * V;
+        if (live && h0 + i + u < h1 && e0 < p.K) {
+          xr[u][j].load(x + (h0 + i + u) * hs + e0);
+          gr[u][j].load(dy + (h0 + i + u) * gs + e0);
+          if (rot[j].on && !(p.pairs && V > 1)) pr[u][j].load(dy + (h0 + i + u) * gs + rot[j].p0);
+        }
       }
-    }
-    ss = group_sum(ss, p.lanes);
-    if (!on) continue;
-    const float s = rsqrtf(ss / (float)p.K + p.eps);
-    const void* w = isq ? p.qw : p.kw;
-    T* y = isq ? static_cast<T*>(p.yq) + (tok * p.H + hh) * p.K : static_cast<T*>(p.yk) + (tok * p.HK + hh) * p.K;
+    float ss[HB], ex[HB];
+    float e[HB][J][V];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int e0 = (l + j * p.lanes) * V;
-      if (e0 < p.K) {
-        float wv[V], out[V];
-        weights<V>(w, p.wdtype, e0, true, wv);
+    for (int u = 0; u < HB; ++u) {
+      ss[u] = ex[u] = 0.f;
 #pragma unroll
-        for (int c = 0; c < V; ++c) out[c] = v[j][c] * s * wv[c];
-        if (rot[j].on) {
-          float o[V];
-          if (p.pairs && V > 1) {
+      for (int j = 0; j < J; ++j) {
+        if (live && h0 + i + u < h1 && (l + j * p.lanes) * V < p.K) {
+          float v[V];
+          xr[u][j].get(v);
+          gr[u][j].get(e[u][j]);
+          if (rot[j].on) {
+            float o[V];
+            if (p.pairs && V > 1) {
 #pragma unroll
-            for (int c = 0; c < V; ++c) o[c] = out[c ^ (V > 1 ? 1 : 0)];
-          } else {
-            float pw[V];
-            Vx<T, V>::load(x + rot[j].p0, o);
-            weights<V>(w, p.wdtype, rot[j].p0, true, pw);
+              for (int c = 0; c < V; ++c) o[c] = e[u][j][c ^ (V > 1 ? 1 : 0)];
+            } else {
+              pr[u][j].get(o);
+            }
 #pragma unroll
-            for (int c = 0; c < V; ++c) o[c] *= s * pw[c];
+            for (int c = 0; c < V; ++c) e[u][j][c] = fmaf(e[u][j][c], rot[j].c[c], o[c] * rot[j].s[c]);
           }
 #pragma unroll
-          for (int c = 0; c < V; ++c) out[c] = fmaf(out[c], rot[j].c[c], o[c] * rot[j].s[c]);
+          for (int c = 0; c < V; ++c) {
+            ss[u] = fmaf(v[c], v[c], ss[u]);
+            ex[u] = fmaf(e[u][j][c] * w[j][c], v[c], ex[u]);
+          }
         }
-        Vx<T, V>::store(y + e0, out);
+      }
+    }
+    for (int o = p.lanes >> 1; o > 0; o >>= 1)
+#pragma unroll
+      for (int u = 0; u < HB; ++u) {
+        ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
+        ex[u] += __shfl_xor_sync(0xffffffffu, ex[u], o);
+      }
+#pragma unroll
+    for (int u = 0; u < HB; ++u) {
+      const float s = rsqrtf(ss[u] / (float)p.K + p.eps);
+      const float m = s * s * ex[u] / (float)p.K;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int e0 = (l + j * p.lanes) * V;
+        if (live && h0 + i + u < h1 && e0 < p.K) {
+          float v[V], out[V];
+          xr[u][j].get(v);
+#pragma unroll
+          for (int c = 0; c < V; ++c) {
+            out[c] = s * (e[u][j][c] * w[j][c] - v[c] * m);
+            dw[j][c] = fmaf(e[u][j][c] * v[c], s, dw[j][c]);
+          }
+          Vx<T, V>::store(dx + (h0 + i + u) * p.K + e0, out);
+        }
       }
     }
   }
 }
 
-// One pass: both sums of a row (x^2 and e x) come from the same loads.  Each block keeps its rows'
-// dw terms and writes one partial row per weight.
+// Each block keeps its rows' dw terms and writes one partial row per weight.
 template <typename T, int V, int J>
 __global__ void __launch_bounds__(256) k_qk_bwd(const P p) {
+  constexpr int HB = J == 1 ? 2 : 1;
   const int lane = threadIdx.x & 31, l = lane & (p.lanes - 1), warp = threadIdx.x >> 5;
   const int rpw = 32 / p.lanes;
   const int64_t units = p.tokens * p.nhg, step = (int64_t)gridDim.x * 8 * rpw;
@@ -175,81 +296,30 @@ __global__ void __launch_bounds__(256) k_qk_bwd(const P p) {
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int c = 0; c < V; ++c) dw[g][j][c] = 0.f;
-  const int heads = p.H + p.HK;
   for (int64_t u0 = first; u0 < units; u0 += step) {  // the same turns for every lane of a warp
     const int64_t unit = u0 + lane / p.lanes;
     const bool live = unit < units;
     const int64_t tok = live ? unit / p.nhg : 0;
-    const int h0 = live ? (int)(unit - tok * p.nhg) * p.hg : 0;
+    const int h0 = live ? (int)(unit - tok * p.nhg) * p.hg : 0, h1 = h0 + p.hg;
     const int b = (int)(tok / p.T), t = (int)(tok - (int64_t)b * p.T);
-    int64_t pos = t;
-    if (p.R && p.pos)
-      pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[b * p.pb + t]
-                    : static_cast<const int32_t*>(p.pos)[b * p.pb + t];
+    const int64_t pos = position(p, b, t);
     Rot<V> rot[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int e0 = (l + j * p.lanes) * V;
       rot[j] = rotation<V>(p, e0 < p.K ? e0 : p.K, pos, -1.f);
     }
-    for (int i = 0; i < p.hg; ++i) {
-      const int h = h0 + i;
-      const bool on = live && h < heads, isq = h < p.H;
-      const int hh = isq ? h : h - p.H;
-      const T* x = isq ? static_cast<const T*>(p.q) + b * p.qs[0] + t * p.qs[1] + hh * p.qs[2]
-                       : static_cast<const T*>(p.k) + b * p.ks[0] + t * p.ks[1] + hh * p.ks[2];
-      const T* dy = isq ? static_cast<const T*>(p.dyq) + b * p.dqs[0] + t * p.dqs[1] + hh * p.dqs[2]
-                        : static_cast<const T*>(p.dyk) + b * p.dks[0] + t * p.dks[1] + hh * p.dks[2];
-      const void* w = isq ? p.qw : p.kw;
-      float v[J][V], e[J][V], ss = 0.f, ex = 0.f;
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int e0 = (l + j * p.lanes) * V;
-        if (on && e0 < p.K) {
-          float wv[V];
-          Vx<T, V>::load(x + e0, v[j]);
-          Vx<T, V>::load(dy + e0, e[j]);
-          if (rot[j].on) {
-            float o[V];
-            if (p.pairs && V > 1) {
-#pragma unroll
-              for (int c = 0; c < V; ++c) o[c] = e[j][c ^ (V > 1 ? 1 : 0)];
-            } else {
-              Vx<T, V>::load(dy + rot[j].p0, o);
-            }
-#pragma unroll
-            for (int c = 0; c < V; ++c) e[j][c] = fmaf(e[j][c], rot[j].c[c], o[c] * rot[j].s[c]);
-          }
-          weights<V>(w, p.wdtype, e0, true, wv);
-#pragma unroll
-          for (int c = 0; c < V; ++c) {
-            ss = fmaf(v[j][c], v[j][c], ss);
-            ex = fmaf(e[j][c] * wv[c], v[j][c], ex);
-          }
-        }
-      }
-      ss = group_sum(ss, p.lanes);
-      ex = group_sum(ex, p.lanes);
-      if (!on) continue;
-      const float s = rsqrtf(ss / (float)p.K + p.eps);
-      const float m = s * s * ex / (float)p.K;
-      T* dx = isq ? static_cast<T*>(p.dq) + (tok * p.H + hh) * p.K : static_cast<T*>(p.dk) + (tok * p.HK + hh) * p.K;
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int e0 = (l + j * p.lanes) * V;
-        if (e0 < p.K) {
-          float wv[V], out[V];
-          weights<V>(w, p.wdtype, e0, true, wv);
-#pragma unroll
-          for (int c = 0; c < V; ++c) {
-            out[c] = s * (e[j][c] * wv[c] - v[j][c] * m);
-            const float d = e[j][c] * v[j][c] * s;
-            if (isq) dw[0][j][c] += d; else dw[1][j][c] += d;
-          }
-          Vx<T, V>::store(dx + e0, out);
-        }
-      }
-    }
+    const int q1 = min(h1, p.H), k0 = max(h0, p.H) - p.H, k1 = min(h1, p.H + p.HK) - p.H;
+    const int qn = __reduce_max_sync(0xffffffffu, live ? max(q1 - h0, 0) : 0);
+    const int kn = __reduce_max_sync(0xffffffffu, live ? max(k1 - k0, 0) : 0);
+    if (qn > 0)
+      heads_bwd<T, V, J, HB>(p, static_cast<const T*>(p.q) + b * p.qs[0] + t * p.qs[1], p.qs[2],
+                             static_cast<const T*>(p.dyq) + b * p.dqs[0] + t * p.dqs[1], p.dqs[2],
+                             static_cast<T*>(p.dq) + tok * p.H * p.K, p.qw, h0, q1, qn, live, l, rot, dw[0]);
+    if (kn > 0)
+      heads_bwd<T, V, J, HB>(p, static_cast<const T*>(p.k) + b * p.ks[0] + t * p.ks[1], p.ks[2],
+                             static_cast<const T*>(p.dyk) + b * p.dks[0] + t * p.dks[1], p.dks[2],
+                             static_cast<T*>(p.dk) + tok * p.HK * p.K, p.kw, k0, k1, kn, live, l, rot, dw[1]);
   }
   if (p.part == nullptr) return;
   // rows of the block: fold the groups of a warp, then the warps, in a fixed order
@@ -317,6 +387,7 @@ P params(const tops_gla_qk_norm_args* a) {
   p.cos = a->cos_table; p.sin = a->sin_table;
   p.pos = a->positions; p.pb = a->positions_stride_b;
   p.yq = a->q_out; p.yk = a->k_out;
+  p.wvec = aligned_to(a->q_weight, 16) && aligned_to(a->k_weight, 16);
   return p;
 }
 

@@ -2,6 +2,8 @@
 // elements of T in as few aligned 16-byte accesses as V allows, fp32 arithmetic between.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace tops {
@@ -40,6 +42,41 @@ struct Vx {
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) p[i] = raw[i];
+    }
+  }
+};
+
+// V elements as they lie in memory, taken apart only where they are used: a load's registers may not be touched before
+template <typename T, int V>
+struct Raw {
+  static constexpr int B = V * (int)sizeof(T);
+  uint32_t w[B >= 4 ? B / 4 : 1];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (B % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < B / 16; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (B == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x; w[1] = v.y;
+    } else if constexpr (B == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void get(float (&r)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        r[i] = __uint_as_float(w[i]);
+      } else {
+        const uint16_t h = (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
+        if constexpr (std::is_same<T, __half>::value) r[i] = __half2float(__ushort_as_half(h));
+        else r[i] = __uint_as_float((uint32_t)h << 16);
+      }
     }
   }
 };

@@ -9,7 +9,7 @@ template <typename T, int LN, int NT, int CH, bool VAR, bool SUM>
 __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
   constexpr int TS = 32, DB = 128 / LN * CH, NP = LN * NT, QC = DB / 4, RPP = 128 / QC, QN = RPP >= TS ? 1 : TS / RPP;
   constexpr int BQ = TS * NP / 4, BN = (BQ + 127) / 128;           // quads of B (of C) in a tile
-  constexpr int RG = LN / CH < 4 ? LN / CH : 4, V = RG * CH;       // rows whose sums are folded at once
+  constexpr int RG = 4, V = RG * CH;                               // rows in flight, whose sums are folded at once
   __shared__ __align__(16) float2 su[TS][DB];
   __shared__ __align__(16) float sb[TS][NP], sc[TS][NP], sy[TS][DB];
   __shared__ int sflag[TS], sseq[TS];
@@ -96,15 +96,11 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
         const bool gone = t0 + row >= t_end || (VAR && (sflag[row] & kNone));
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          float f[4];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float dl = dr[j].get(i + e) + bias[i + e];
-            if (p.softplus) dl = softplus(dl);
-            f[2 * e] = gone ? 0.f : dl;
-            f[2 * e + 1] = gone ? 0.f : dl * xr[j].get(i + e);
-          }
-          *reinterpret_cast<float4*>(&su[row][qc * 4 + i]) = make_float4(f[0], f[1], f[2], f[3]);
+          float2 dl = make_float2(dr[j].get(i) + bias[i], dr[j].get(i + 1) + bias[i + 1]);
+          if (p.softplus) dl = softplus2(dl);
+          if (gone) dl = dup(0.f);
+          *reinterpret_cast<float4*>(&su[row][qc * 4 + i]) =
+              make_float4(dl.x, gone ? 0.f : dl.x * xr[j].get(i), dl.y, gone ? 0.f : dl.y * xr[j].get(i + 1));
         }
       }
     }
@@ -135,6 +131,30 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
           if (c0 + cb + i < rep)
             states_store<NT>(p.states + (((int64_t)b * nck + (t0 + r0) / CK) * p.D + dbase + cb + i) * p.N, n0, p.N, h[i]);
       }
+      // the decays and inputs of all rows first: nothing of them waits for a state
+      float2 a[RG][CH][NT / 2], ub[RG][CH][NT / 2];
+#pragma unroll
+      for (int rr = 0; rr < RG; ++rr) {
+        float2 Bv[NT / 2];
+        pairs_load<NT>(&sb[r0 + rr][n0], Bv);
+        float du[2 * CH];
+        if constexpr (CH == 2) {
+          const float4 q = *reinterpret_cast<const float4*>(&su[r0 + rr][cb]);
+          du[0] = q.x; du[1] = q.y; du[2] = q.z; du[3] = q.w;
+        } else {
+          const float2 q = su[r0 + rr][cb];
+          du[0] = q.x; du[1] = q.y;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          if (SUM) dsum[i] += du[2 * i];
+#pragma unroll
+          for (int j = 0; j < NT / 2; ++j) {
+            a[rr][i][j] = decay2(du[2 * i], A[i][j]);
+            ub[rr][i][j] = mul2(dup(du[2 * i + 1]), Bv[j]);
+          }
+        }
+      }
       float ys[V];
 #pragma unroll
       for (int rr = 0; rr < RG; ++rr) {
@@ -152,27 +172,17 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
             }
           }
         }
-        float2 Bv[NT / 2], Cv[NT / 2];
-        pairs_load<NT>(&sb[r][n0], Bv);
+        float2 Cv[NT / 2];
         if (!SUM) pairs_load<NT>(&sc[r][n0], Cv);
-        float du[2 * CH];
-        if constexpr (CH == 2) {
-          const float4 q = *reinterpret_cast<const float4*>(&su[r][cb]);
-          du[0] = q.x; du[1] = q.y; du[2] = q.z; du[3] = q.w;
-        } else {
-          const float2 q = su[r][cb];
-          du[0] = q.x; du[1] = q.y;
-        }
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           float2 acc = dup(0.f);
 #pragma unroll
           for (int j = 0; j < NT / 2; ++j) {
-            h[i][j] = fma2(decay2(du[2 * i], A[i][j]), h[i][j], mul2(dup(du[2 * i + 1]), Bv[j]));
+            h[i][j] = fma2(a[rr][i][j], h[i][j], ub[rr][i][j]);
             if (!SUM) acc = j ? fma2(Cv[j], h[i][j], acc) : mul2(Cv[j], h[i][j]);
           }
-          if (SUM) dsum[i] += du[2 * i];
-          else ys[rr * CH + i] = acc.x + acc.y;
+          if (!SUM) ys[rr * CH + i] = acc.x + acc.y;
         }
         if (VAR && !SUM && (f & kLast) && p.ht) {
 #pragma unroll
@@ -225,28 +235,78 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
   if (SUM && VAR && blockIdx.x == 0 && tid == 0) p.broken[k] = broken != 0;
 }
 
-// One token of each of B rows: the state is read and written once (HBM bounds it).
-template <typename T>
-__global__ void __launch_bounds__(128) k_scan_step(const P p) {
-  const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
-  if (id >= (int64_t)p.B * p.D) return;
-  const int b = (int)(id / p.D), d = (int)(id - (int64_t)b * p.D), grp = d / (p.D / p.G);
-  const float x = to_f<T>(static_cast<const T*>(p.x)[b * p.xs[0] + d]);
-  float dl = to_f<T>(static_cast<const T*>(p.dt)[b * p.ds[0] + d]) + (p.bias ? p.bias[d] : 0.f);
-  if (p.softplus) dl = softplus(dl);
-  const T* Bt = static_cast<const T*>(p.bm) + b * p.bs[0] + grp * p.N;
-  const T* Ct = static_cast<const T*>(p.cm) + b * p.cs[0] + grp * p.N;
-  float y = p.skip ? p.skip[d] * x : 0.f;
-  for (int n = 0; n < p.N; ++n) {
-    const float h = fmaf(__expf(dl * p.A[(int64_t)d * p.N + n]), p.h0[id * p.N + n], dl * x * to_f<T>(Bt[n]));
-    p.ht[id * p.N + n] = h;
-    y = fmaf(to_f<T>(Ct[n]), h, y);
+// One token of each of B rows: the state is read and written once (HBM bounds it).  Q lanes share a channel, four
+// states each (16 bytes of the state), and take R rows of the batch one after another, their states loaded together:
+// A, the bias and the skip weight are read once for them.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_scan_step(const P p, int Q, int R) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, ch = id / Q;
+  const int nq = (int)(id - ch * Q), n0 = nq * 4;
+  const bool on = ch < p.D;
+  const int d = on ? (int)ch : 0, grp = d / (p.D / p.G), cnt = min(4, p.N - n0);
+  float A[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) A[i] = on && i < cnt ? p.A[(int64_t)d * p.N + n0 + i] * kLog2e : 0.f;
+  const float bias = p.bias ? p.bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
+  const int b0 = blockIdx.y * R;
+  constexpr int U = 4;
+  for (int bb = b0; bb < min(b0 + R, p.B); bb += U) {
+    float h[U][4];
+    float x[U], dt[U], z[U], Bv[U][4], Cv[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = bb + u;
+      const bool row = on && cnt > 0 && b < min(b0 + R, p.B);
+      const float* hp = p.h0 + ((int64_t)b * p.D + d) * p.N + n0;
+      if (VEC) {
+        const float4 v = row ? *reinterpret_cast<const float4*>(hp) : make_float4(0.f, 0.f, 0.f, 0.f);
+        h[u][0] = v.x; h[u][1] = v.y; h[u][2] = v.z; h[u][3] = v.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[u][i] = row && i < cnt ? hp[i] : 0.f;
+      }
+      x[u] = row ? to_f<T>(static_cast<const T*>(p.x)[b * p.xs[0] + d]) : 0.f;
+      dt[u] = row ? to_f<T>(static_cast<const T*>(p.dt)[b * p.ds[0] + d]) : 0.f;
+      z[u] = row && p.z ? to_f<T>(static_cast<const T*>(p.z)[b * p.zs[0] + d]) : 0.f;
+      Quad<T> bq, cq;
+      quad_load<T>(static_cast<const T*>(p.bm) + b * p.bs[0] + grp * p.N + n0, p.vb, row ? cnt : 0, bq);
+      quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + grp * p.N + n0, p.vc, row ? cnt : 0, cq);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        Bv[u][i] = bq.get(i);
+        Cv[u][i] = cq.get(i);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = bb + u;
+      const bool row = on && cnt > 0 && b < min(b0 + R, p.B);
+      float dl = dt[u] + bias;
+      if (p.softplus) dl = softplus(dl);
+      const float du = dl * x[u];
+      float y = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        h[u][i] = fmaf(ex2(fmaf(dl, A[i], kEx2Mean)), h[u][i], du * Bv[u][i]);
+        y = fmaf(Cv[u][i], h[u][i], y);
+      }
+      for (int o = 1; o < Q; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (!row) continue;
+      float* ho = p.ht + ((int64_t)b * p.D + d) * p.N + n0;
+      if (VEC) {
+        *reinterpret_cast<float4*>(ho) = make_float4(h[u][0], h[u][1], h[u][2], h[u][3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < cnt) ho[i] = h[u][i];
+      }
+      if (nq == 0) {
+        y = fmaf(skip, x[u], y);
+        if (p.z) y *= z[u] * fast_sigmoid(z[u]);
+        static_cast<T*>(p.y)[(int64_t)b * p.D + d] = from_f<T>(y);
+      }
+    }
   }
-  if (p.z) {
-    const float z = to_f<T>(static_cast<const T*>(p.z)[b * p.zs[0] + d]);
-    y *= z * fast_sigmoid(z);
-  }
-  static_cast<T*>(p.y)[id] = from_f<T>(y);
 }
 
 // channels of a forward thread: two share the loads of B and C
@@ -323,8 +383,19 @@ TOPS_API int tops_gla_ssm_scan_step(const tops_gla_scan_args* a, void* stream) {
   const P p = params(a);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchTimer lt(st, "ssm_scan_step");
+  int Q = 1;  // lanes of a channel: a power of two, so that a channel lies in one warp
+  while (Q * 4 < p.N) Q *= 2;
+  const int blocks = (int)(((int64_t)p.D * Q + 255) / 256);
+  // rows of a thread: all loads of four are in flight at once; fewer where the grid would not fill the SMs
+  int R = 4;
+  while (R > 1 && (int64_t)blocks * ((p.B + R - 1) / R) < 148 * 4) R /= 2;
+  R = std::max(R, (p.B + 65534) / 65535);
+  const bool vec = p.N % 4 == 0 && aligned_to(p.h0, 16) && aligned_to(p.ht, 16);
   by_type(a->dtype, [&](auto t) {
-    k_scan_step<decltype(t)><<<(unsigned)(((int64_t)p.B * p.D + 127) / 128), 128, 0, st>>>(p);
+    using T = decltype(t);
+    const dim3 grid(blocks, (p.B + R - 1) / R);
+    if (vec) k_scan_step<T, true><<<grid, 256, 0, st>>>(p, Q, R);
+    else k_scan_step<T, false><<<grid, 256, 0, st>>>(p, Q, R);
     return 0;
   });
   TOPS_CUDA_LAUNCH_CHECK("ssm_scan_step");

@@ -88,7 +88,24 @@ __device__ __forceinline__ float2 decay2(float delta, float2 A) {
   return make_float2(ex2(e.x), ex2(e.y));
 }
 
-__device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1pf(__expf(v)); }
+// softplus(v) = max(v, 0) + log1p(w), w = exp(-|v|) in (0, 1], of a pair.  log1p(w) = w q(w) with q the interpolant of
+// log1p(w) / w in ten Chebyshev nodes of [0, 1]: off by 1e-7 relative (in fp32, also for the smallest w), nine packed
+// multiply-adds for two channels and no second use of the exponential unit.
+__device__ __forceinline__ float2 softplus2(float2 v) {
+  const float2 w = make_float2(ex2(-kLog2e * fabsf(v.x)), ex2(-kLog2e * fabsf(v.y)));
+  float2 q = dup(-3.176057013e-03f);
+  q = fma2(q, w, dup(1.954252832e-02f));
+  q = fma2(q, w, dup(-5.637361482e-02f));
+  q = fma2(q, w, dup(1.054362357e-01f));
+  q = fma2(q, w, dup(-1.526966691e-01f));
+  q = fma2(q, w, dup(1.966327429e-01f));
+  q = fma2(q, w, dup(-2.495161593e-01f));
+  q = fma2(q, w, dup(3.332971036e-01f));
+  q = fma2(q, w, dup(-4.999989271e-01f));
+  q = fma2(q, w, dup(1.f));
+  return fma2(w, q, make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
+}
+__device__ __forceinline__ float softplus(float v) { return softplus2(make_float2(v, v)).x; }
 
 // Sums of V values over the L lanes that differ in bits m0, 2 m0, ... of the lane: as long as a lane carries
 // several, an exchange halves them.  Returns the first index of the V >> log2(L) (at least one) that this lane holds.

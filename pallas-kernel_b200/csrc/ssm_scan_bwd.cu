@@ -90,10 +90,17 @@ __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
     const bool gone = qr >= TS || t0 + qr >= t_end || (VAR && (sflag[qr] & kNone));
     float xf[4], vf[4], zf[4], gf[4], dl[4], dy[4], zs[4];  // kept for the tile's outputs
 #pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      vf[i] = dr.get(i) + bias[i];
+      vf[i + 1] = dr.get(i + 1) + bias[i + 1];
+      float2 v = make_float2(vf[i], vf[i + 1]);
+      if (p.softplus) v = softplus2(v);
+      dl[i] = gone ? 0.f : v.x;
+      dl[i + 1] = gone ? 0.f : v.y;
+    }
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
       xf[i] = gone ? 0.f : xr.get(i);
-      vf[i] = dr.get(i) + bias[i];
-      dl[i] = gone ? 0.f : p.softplus ? softplus(vf[i]) : vf[i];
       gf[i] = gone ? 0.f : gr.get(i);
       zf[i] = gone ? 0.f : zr.get(i);
       zs[i] = fast_sigmoid(zf[i]);
@@ -331,12 +338,16 @@ __global__ void __launch_bounds__(128) k_scan_bwd_sum(const P p) {
       float f[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float dl = dr.get(i) + bias[i];
-        if (p.softplus) dl = softplus(dl);
         const float z = zr.get(i);
         const float dy = p.z ? gr.get(i) * z * fast_sigmoid(z) : gr.get(i);
-        f[2 * i] = gone ? 0.f : dl;
         f[2 * i + 1] = gone ? 0.f : dy;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        float2 dl = make_float2(dr.get(i) + bias[i], dr.get(i + 1) + bias[i + 1]);
+        if (p.softplus) dl = softplus2(dl);
+        f[2 * i] = gone ? 0.f : dl.x;
+        f[2 * i + 2] = gone ? 0.f : dl.y;
       }
       *reinterpret_cast<float4*>(&su[row][qc * 4]) = make_float4(f[0], f[1], f[2], f[3]);
       *reinterpret_cast<float4*>(&su[row][qc * 4 + 2]) = make_float4(f[4], f[5], f[6], f[7]);
