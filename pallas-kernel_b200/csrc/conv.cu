@@ -34,7 +34,7 @@ struct P {
   int strip, strips, dv;  // rows of a strip, strips of one batch row, column groups
 };
 
-__device__ __forceinline__ float act_fwd(float p, int act) { return act ? __fdividef(p, 1.f + __expf(-p)) : p; }
+__device__ __forceinline__ float act_fwd(float p, int act) { return act ? p * fast_sigmoid(p) : p; }
 __device__ __forceinline__ float act_grad(float p, int act) {
   if (!act) return 1.f;
   const float s = fast_sigmoid(p);
@@ -71,6 +71,22 @@ __device__ __forceinline__ void load_params(const P& p, int d0, float (&w)[W][V]
     for (int j = 0; j < W; ++j) w[j][i] = flat[(i * W + j) / V][(i * W + j) % V];
 }
 
+// Rows on their way: every thread copies the vectors that it will use itself into its own column of shared memory, so
+// that several batches of R rows are in flight without registers and no thread waits for another.
+constexpr int R = 4;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  const uint32_t a = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(a), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int AHEAD>
+__device__ __forceinline__ void copies_wait() {  // all but the last AHEAD groups have arrived
+  asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
+}
+
 // the sequence of row t of batch row b: [s, e) and its number (-1: none)
 __device__ __forceinline__ SeqAt seq_of(const P& p, int b, int t) {
   if (p.cu == nullptr) return SeqAt{b, 0, p.T};
@@ -90,6 +106,22 @@ __device__ __forceinline__ void row_or_state(const P& p, int b, const SeqAt& q, 
 #pragma unroll
     for (int i = 0; i < V; ++i) r[i] = 0.f;
   }
+}
+
+// p of a row from its window
+template <int V, int W>
+__device__ __forceinline__ void sum_of(const float (&w)[W][V], const float (&bias)[V], const float (&win)[W][V], float (&a)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) a[i] = bias[i];
+#pragma unroll
+  for (int j = 0; j < W; ++j) fma_n<V>(a, w[j], win[j]);
+}
+template <int V, int W>
+__device__ __forceinline__ void act_of(const P& p, const float (&w)[W][V], const float (&bias)[V],
+                                       const float (&win)[W][V], float (&out)[V]) {
+  sum_of<V, W>(w, bias, win, out);
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = act_fwd(out[i], p.act);
 }
 
 // final state of sequence n, channels d0..: its last W - 1 inputs
@@ -114,7 +146,6 @@ __device__ void final_state(const P& p, int n, int d0) {
 
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
-  constexpr int R = 4;
   const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
   const int64_t unit = id / p.dv;
   const int d0 = (int)(id - unit * p.dv) * V;
@@ -155,52 +186,46 @@ __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
       for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
     Vx<T, V>::load(x + t * p.xt, win[W - 1]);
     float out[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float a = bias[i];
-#pragma unroll
-      for (int j = 0; j < W; ++j) a = fmaf(w[j][i], win[j][i], a);
-      out[i] = act_fwd(a, p.act);
-    }
+    act_of<V, W>(p, w, bias, win, out);
     Vx<T, V>::store(y + (int64_t)t * p.D, out);
   };
-  // R rows inside one sequence: their loads are issued R rows ahead of their use
-  Raw<T, V> next[R];
-  int have = -1;  // first row in `next`
-  for (int t = t0; t < t1;) {
-    if (t + R > t1 || t + R > q.e || q.n < 0) {
-      row(t++);
-      continue;
-    }
-    if (have != t)
+  if constexpr (V == 1) {
+    for (int t = t0; t < t1; ++t) row(t);
+    return;
+  } else {
+    constexpr int kAhead = 3, kSlots = R * (kAhead + 1);
+    __shared__ Raw<T, V> ring[kSlots][128];
+    const int batches = (t1 - t0) / R;
+    auto ask = [&](int g) {
+      if (g < batches)
 #pragma unroll
-      for (int r = 0; r < R; ++r) next[r].load(x + (t + r) * p.xt);
-    Raw<T, V> cur[R];
+        for (int r = 0; r < R; ++r)
+          copy_async<Raw<T, V>::B>(&ring[(g * R + r) % kSlots][threadIdx.x], x + (t0 + g * R + r) * p.xt);
+      copies_commit();
+    };
 #pragma unroll
-    for (int r = 0; r < R; ++r) cur[r] = next[r];
-    if (t + 2 * R <= t1) {
-      have = t + R;
-#pragma unroll
-      for (int r = 0; r < R; ++r) next[r].load(x + (t + R + r) * p.xt);
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-      for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
-      cur[r].get(win[W - 1]);
-      float out[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float a = bias[i];
-#pragma unroll
-        for (int j = 0; j < W; ++j) a = fmaf(w[j][i], win[j][i], a);
-        out[i] = act_fwd(a, p.act);
+    for (int g = 0; g < kAhead; ++g) ask(g);
+    for (int g = 0; g < batches; ++g) {
+      ask(g + kAhead);
+      copies_wait<kAhead>();
+      const int t = t0 + g * R;
+      if (t + R > q.e || q.n < 0) {  // a sequence ends here
+        for (int r = 0; r < R; ++r) row(t + r);
+        continue;
       }
-      Vx<T, V>::store(y + (int64_t)(t + r) * p.D, out);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
+        ring[(g * R + r) % kSlots][threadIdx.x].get(win[W - 1]);
+        float out[V];
+        act_of<V, W>(p, w, bias, win, out);
+        Vx<T, V>::store(y + (int64_t)(t + r) * p.D, out);
+      }
     }
-    t += R;
+    for (int t = t0 + batches * R; t < t1; ++t) row(t);
   }
 }
 
@@ -208,13 +233,11 @@ __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
 template <int V, int W>
 __device__ __forceinline__ void dp_of(const P& p, const float (&w)[W][V], const float (&bias)[V],
                                       const float (&win)[W][V], float (&dp)[V]) {
+  float a[V];
+  sum_of<V, W>(w, bias, win, a);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float a = bias[i];
-#pragma unroll
-    for (int j = 0; j < W; ++j) a = fmaf(w[j][i], win[j][i], a);
-    dp[i] *= act_grad(a, p.act);
-  }
+  for (int i = 0; i < V; ++i) a[i] = act_grad(a[i], p.act);
+  mul_n<V>(dp, dp, a);
 }
 
 // Gradient of sequence n's carried state, channels d0..: its column c is read by the rows
@@ -268,7 +291,6 @@ __device__ void state_grad(const P& p, const float (&w)[W][V], const float (&bia
 // strip, whose rows alone go into dw and db).
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
-  constexpr int R = 4;
   const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
   const int64_t unit = id / p.dv;
   const int d0 = (int)(id - unit * p.dv) * V;
@@ -339,61 +361,59 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
     }
     if (t - (W - 1) >= t0) Vx<T, V>::store(dx + (int64_t)(t - (W - 1)) * p.D, acc[W - 1]);
   };
-  // R rows inside one sequence, W - 1 rows or more from either end of it and inside the strip: their loads are
-  // issued R rows ahead of their use
-  Raw<T, V> nx[R], ng[R];
-  int have = -1;
-  for (int t = t0; t < t1 + W - 1;) {
-    if (q.n < 0 || t < max(q.s, t0) + W - 1 || t + R > min(t1, q.e - (W - 1))) {
-      row(t++);
-      continue;
-    }
-    if (have != t)
+  const int stop = t1 + W - 1;
+  if constexpr (V == 1) {
+    for (int t = t0; t < stop; ++t) row(t);
+  } else {
+    constexpr int kAhead = Raw<T, V>::B == 16 ? 1 : 3, kSlots = R * (kAhead + 1);  // 32 KB
+    __shared__ Raw<T, V> ring[2][kSlots][128];
+    const int batches = (t1 - t0) / R;
+    auto ask = [&](int g) {
+      if (g < batches)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int t = t0 + g * R + r, at = (g * R + r) % kSlots;
+          copy_async<Raw<T, V>::B>(&ring[0][at][threadIdx.x], x + t * p.xt);
+          copy_async<Raw<T, V>::B>(&ring[1][at][threadIdx.x], dy + t * p.gt);
+        }
+      copies_commit();
+    };
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) ask(g);
+    for (int g = 0; g < batches; ++g) {
+      ask(g + kAhead);
+      copies_wait<kAhead>();
+      const int t = t0 + g * R;
+      // fewer than W - 1 rows from the strip's begin or from an end of the sequence
+      if (q.n < 0 || t < max(q.s, t0) + W - 1 || t + R > q.e - (W - 1)) {
+        for (int r = 0; r < R; ++r) row(t + r);
+        continue;
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        nx[r].load(x + (t + r) * p.xt);
-        ng[r].load(dy + (t + r) * p.gt);
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
+#pragma unroll
+        for (int j = W - 1; j > 0; --j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[j][i] = acc[j - 1][i];
+        float dp[V];
+        ring[0][(g * R + r) % kSlots][threadIdx.x].get(win[W - 1]);
+        ring[1][(g * R + r) % kSlots][threadIdx.x].get(dp);
+        dp_of<V, W>(p, w, bias, win, dp);
+        mul_n<V>(acc[0], w[W - 1], dp);
+#pragma unroll
+        for (int k = 1; k < W; ++k) fma_n<V>(acc[k], w[W - 1 - k], dp);
+#pragma unroll
+        for (int i = 0; i < V; ++i) db[i] += dp[i];
+#pragma unroll
+        for (int j = 0; j < W; ++j) fma_n<V>(dw[j], dp, win[j]);
+        Vx<T, V>::store(dx + (int64_t)(t + r - (W - 1)) * p.D, acc[W - 1]);
       }
-    Raw<T, V> cx[R], cg[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      cx[r] = nx[r];
-      cg[r] = ng[r];
     }
-    if (t + 2 * R <= t1) {
-      have = t + R;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        nx[r].load(x + (t + R + r) * p.xt);
-        ng[r].load(dy + (t + R + r) * p.gt);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-      for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
-#pragma unroll
-      for (int j = W - 1; j > 0; --j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[j][i] = acc[j - 1][i];
-      float dp[V];
-      cx[r].get(win[W - 1]);
-      cg[r].get(dp);
-      dp_of<V, W>(p, w, bias, win, dp);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        acc[0][i] = w[W - 1][i] * dp[i];
-#pragma unroll
-        for (int k = 1; k < W; ++k) acc[k][i] = fmaf(w[W - 1 - k][i], dp[i], acc[k][i]);
-        db[i] += dp[i];
-#pragma unroll
-        for (int j = 0; j < W; ++j) dw[j][i] = fmaf(dp[i], win[j][i], dw[j][i]);
-      }
-      Vx<T, V>::store(dx + (int64_t)(t + r - (W - 1)) * p.D, acc[W - 1]);
-    }
-    t += R;
+    for (int t = t0 + batches * R; t < stop; ++t) row(t);
   }
   if (p.part != nullptr) {
     float* o = p.part + unit * (W + 1) * p.D + d0;

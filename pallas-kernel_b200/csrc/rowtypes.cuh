@@ -50,7 +50,7 @@ struct Vx {
 template <typename T, int V>
 struct Raw {
   static constexpr int B = V * (int)sizeof(T);
-  uint32_t w[B >= 4 ? B / 4 : 1];
+  alignas(B >= 16 ? 16 : B >= 4 ? B : 4) uint32_t w[B >= 4 ? B / 4 : 1];
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (B % 16 == 0) {
 #pragma unroll
@@ -93,7 +93,64 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-__device__ __forceinline__ float fast_sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+constexpr float kLog2e = 1.44269504088896341f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
+// d += a b, d = a b over V elements, two at a time
+template <int V>
+__device__ __forceinline__ void fma_n(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) {
+    d[0] = fmaf(a[0], b[0], d[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = fma2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), make_float2(d[i], d[i + 1]));
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_n(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) {
+    d[0] = a[0] * b[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = mul2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  }
+}
+
+// 1 / (1 + exp(-x)): both hardware approximations, off by at most 2^-22 each; 0 and 1 at the infinities
+__device__ __forceinline__ float fast_sigmoid(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(-kLog2e * x)));
+  return r;
+}
 
 // ---------------------------------------------------------------------------
 // packed sequences: rows [cu[n], cu[n+1]) of one axis of T rows.  The offsets lie on the

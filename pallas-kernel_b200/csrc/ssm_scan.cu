@@ -5,40 +5,38 @@ namespace tops {
 namespace ssm {
 
 // SUM: the first pass over a segment (its state from zero and the sum of delta) instead of its output.
-template <typename T, int LN, int NT, int CH, bool VAR, bool SUM>
-__global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
-  constexpr int TS = 32, DB = 128 / LN * CH, NP = LN * NT, QC = DB / 4, RPP = 128 / QC, QN = RPP >= TS ? 1 : TS / RPP;
-  constexpr int BQ = TS * NP / 4, BN = (BQ + 127) / 128;           // quads of B (of C) in a tile
-  constexpr int RG = 4, V = RG * CH;                               // rows in flight, whose sums are folded at once
+constexpr int kFwdThreads = 128;
+
+template <typename T, int LN, int NT, bool VAR, bool SUM>
+__global__ void __launch_bounds__(kFwdThreads) k_scan_fwd(const P p) {
+  constexpr int TS = 32, DB = kFwdThreads / LN, NP = LN * NT, QC = DB / 4, RPP = kFwdThreads / QC;
+  constexpr int QN = RPP >= TS ? 1 : TS / RPP, NH = NT / 2;
+  constexpr int BQ = TS * NP / 4, BN = (BQ + kFwdThreads - 1) / kFwdThreads;           // quads of B (of C) in a tile
+  constexpr int RG = 8;                                            // rows in flight, whose sums are folded at once
   __shared__ __align__(16) float2 su[TS][DB];
   __shared__ __align__(16) float sb[TS][NP], sc[TS][NP], sy[TS][DB];
   __shared__ int sflag[TS], sseq[TS];
   const int tid = threadIdx.x, lane = tid & 31, nl = lane % LN, b = blockIdx.y, k = blockIdx.z;
   const int rep = p.D / p.G, nblk = (rep + DB - 1) / DB, grp = blockIdx.x / nblk;
   const int c0 = (blockIdx.x - grp * nblk) * DB;                   // first channel of the block in its group
-  const int cb = tid / 32 * (32 / LN * CH) + lane / LN * CH;       // first channel of the thread in the block
+  const int cb = tid / 32 * (32 / LN) + lane / LN;                 // channel of the thread in the block
   const int n0 = nl * NT;
   const int64_t dbase = (int64_t)grp * rep + c0;
   const int t_first = k * p.seg, t_end = min(t_first + p.seg, p.T);
 
-  float2 A[CH][NT / 2], h[CH][NT / 2];
-  float dsum[CH];
+  const bool on = c0 + cb < rep;
+  const int64_t d = dbase + cb;
+  float2 A[NH], h[NH];
+  float dsum = 0.f;
+  states_load<NT>(p.A + d * p.N, n0, on ? p.N : 0, A);
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    dsum[i] = 0.f;
-    const bool on = c0 + cb + i < rep;
-    states_load<NT>(p.A + (dbase + cb + i) * p.N, n0, on ? p.N : 0, A[i]);
-#pragma unroll
-    for (int j = 0; j < NT / 2; ++j) {
-      A[i][j] = mul2(A[i][j], dup(kLog2e));
-      h[i][j] = dup(0.f);
-    }
-    if (on && !SUM) {
-      if (k > 0) states_load<NT>(p.carry + (((int64_t)b * p.nseg + k) * p.D + dbase + cb + i) * p.N, n0, p.N, h[i]);
-      else if (!VAR && p.h0) states_load<NT>(p.h0 + ((int64_t)b * p.D + dbase + cb + i) * p.N, n0, p.N, h[i]);
-    }
-    if (on && SUM && !VAR && k == 0 && p.h0)
-      states_load<NT>(p.h0 + ((int64_t)b * p.D + dbase + cb + i) * p.N, n0, p.N, h[i]);
+  for (int j = 0; j < NH; ++j) {
+    A[j] = mul2(A[j], dup(kLog2e));
+    h[j] = dup(0.f);
+  }
+  if (on) {
+    if (k > 0 && !SUM) states_load<NT>(p.carry + (((int64_t)b * p.nseg + k) * p.D + d) * p.N, n0, p.N, h);
+    else if (k == 0 && !VAR && p.h0) states_load<NT>(p.h0 + ((int64_t)b * p.D + d) * p.N, n0, p.N, h);
   }
 
   // staging: this thread's quads of channels are column qc of rows qr, qr + RPP, ...
@@ -68,7 +66,7 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
     }
 #pragma unroll
     for (int j = 0; j < BN; ++j) {
-      const int q = tid + j * 128, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4, t = t0 + row;
+      const int q = tid + j * kFwdThreads, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4, t = t0 + row;
       const int v = (q < BQ && t < t_end) ? min(max(p.N - n, 0), 4) : 0;
       quad_load<T>(bp + t * p.bs[1] + n, p.vb, v, br[j]);
       if (!SUM) quad_load<T>(cp + t * p.cs[1] + n, p.vc, v, cr[j]);
@@ -79,12 +77,14 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
   fetch(t_first);
   int broken = 0;
   for (int t0 = t_first; t0 < t_end; t0 += TS) {
+    bool flagged = false;  // a row of the tile begins or ends a sequence, or belongs to none
     if (VAR) {
       if (tid < TS) {
         sflag[tid] = flag;
         sseq[tid] = seq;
       }
-      broken |= __syncthreads_or(flag & (kFirst | kNone));
+      flagged = __syncthreads_or(flag);
+      if (SUM && flagged) broken |= __syncthreads_or(flag & (kFirst | kNone));
     }
     Quad<T> xc[QN], zc[QN];
 #pragma unroll
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
     }
 #pragma unroll
     for (int j = 0; j < BN; ++j) {
-      const int q = tid + j * 128, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4;
+      const int q = tid + j * kFwdThreads, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4;
       if (q < BQ) {
         const bool gone = VAR && (sflag[row] & kNone);
         float fb[4], fc[4];
@@ -123,77 +123,74 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
     if (t0 + TS < t_end) fetch(t0 + TS);
     const int rows = min(TS, t_end - t0);
 
-    for (int r0 = 0; r0 < rows; r0 += RG) {  // rows at t_end and beyond: delta = 0, nothing moves
-      if (!SUM && p.states != nullptr && (r0 & (CK - 1)) == 0) {
+    auto save = [&](int r) {
+      if (!SUM && p.states != nullptr && on && (r & (CK - 1)) == 0) {
         const int nck = (p.T + CK - 1) / CK;
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-          if (c0 + cb + i < rep)
-            states_store<NT>(p.states + (((int64_t)b * nck + (t0 + r0) / CK) * p.D + dbase + cb + i) * p.N, n0, p.N, h[i]);
+        states_store<NT>(p.states + (((int64_t)b * nck + (t0 + r) / CK) * p.D + d) * p.N, n0, p.N, h);
       }
-      // the decays and inputs of all rows first: nothing of them waits for a state
-      float2 a[RG][CH][NT / 2], ub[RG][CH][NT / 2];
+    };
+    if (VAR && flagged) {  // row by row: few tiles of a packed batch
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r) {
+        save(r);
+        const int f = sflag[r];
+        if (f & (kFirst | kNone)) {
 #pragma unroll
-      for (int rr = 0; rr < RG; ++rr) {
-        float2 Bv[NT / 2];
-        pairs_load<NT>(&sb[r0 + rr][n0], Bv);
-        float du[2 * CH];
-        if constexpr (CH == 2) {
-          const float4 q = *reinterpret_cast<const float4*>(&su[r0 + rr][cb]);
-          du[0] = q.x; du[1] = q.y; du[2] = q.z; du[3] = q.w;
-        } else {
-          const float2 q = su[r0 + rr][cb];
-          du[0] = q.x; du[1] = q.y;
+          for (int j = 0; j < NH; ++j) h[j] = dup(0.f);
+          if ((f & kFirst) && p.h0 && on) states_load<NT>(p.h0 + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, h);
         }
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          if (SUM) dsum[i] += du[2 * i];
-#pragma unroll
-          for (int j = 0; j < NT / 2; ++j) {
-            a[rr][i][j] = decay2(du[2 * i], A[i][j]);
-            ub[rr][i][j] = mul2(dup(du[2 * i + 1]), Bv[j]);
-          }
-        }
-      }
-      float ys[V];
-#pragma unroll
-      for (int rr = 0; rr < RG; ++rr) {
-        const int r = r0 + rr;
-        int f = 0;
-        if (VAR) {
-          f = sflag[r];
-          if (f & (kFirst | kNone)) {
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-#pragma unroll
-              for (int j = 0; j < NT / 2; ++j) h[i][j] = dup(0.f);
-              if ((f & kFirst) && p.h0 && c0 + cb + i < rep)
-                states_load<NT>(p.h0 + ((int64_t)sseq[r] * p.D + dbase + cb + i) * p.N, n0, p.N, h[i]);
-            }
-          }
-        }
-        float2 Cv[NT / 2];
+        float2 Bv[NH], Cv[NH], acc = dup(0.f);
+        pairs_load<NT>(&sb[r][n0], Bv);
         if (!SUM) pairs_load<NT>(&sc[r][n0], Cv);
+        const float2 q = su[r][cb];
+        if (SUM) dsum += q.x;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          float2 acc = dup(0.f);
-#pragma unroll
-          for (int j = 0; j < NT / 2; ++j) {
-            h[i][j] = fma2(a[rr][i][j], h[i][j], ub[rr][i][j]);
-            if (!SUM) acc = j ? fma2(Cv[j], h[i][j], acc) : mul2(Cv[j], h[i][j]);
-          }
-          if (!SUM) ys[rr * CH + i] = acc.x + acc.y;
+        for (int j = 0; j < NH; ++j) {
+          h[j] = fma2(decay2(q.x, A[j]), h[j], mul2(dup(q.y), Bv[j]));
+          if (!SUM) acc = j ? fma2(Cv[j], h[j], acc) : mul2(Cv[j], h[j]);
         }
-        if (VAR && !SUM && (f & kLast) && p.ht) {
-#pragma unroll
-          for (int i = 0; i < CH; ++i)
-            if (c0 + cb + i < rep) states_store<NT>(p.ht + ((int64_t)sseq[r] * p.D + dbase + cb + i) * p.N, n0, p.N, h[i]);
+        if (!SUM) {
+          float y[1] = {acc.x + acc.y};
+          fold<1, LN, 1>(y, lane);
+          sy[r][cb] = y[0];
+          if ((f & kLast) && p.ht && on) states_store<NT>(p.ht + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, h);
         }
       }
-      if (!SUM) {
-        const int at = fold<V, LN, 1>(ys, lane);
+    } else {
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += RG) {  // rows at t_end and beyond: delta = 0, nothing moves
+        save(r0);
+        // the decays and inputs of all rows first: nothing of them waits for a state
+        float2 a[RG][NH], ub[RG][NH];
 #pragma unroll
-        for (int i = 0; i < (V > LN ? V / LN : 1); ++i) sy[r0 + (at + i) / CH][cb + (at + i) % CH] = ys[i];
+        for (int rr = 0; rr < RG; ++rr) {
+          float2 Bv[NH];
+          pairs_load<NT>(&sb[r0 + rr][n0], Bv);
+          const float2 q = su[r0 + rr][cb];
+          if (SUM) dsum += q.x;
+#pragma unroll
+          for (int j = 0; j < NH; ++j) {
+            a[rr][j] = decay2(q.x, A[j]);
+            ub[rr][j] = mul2(dup(q.y), Bv[j]);
+          }
+        }
+        float ys[RG];
+#pragma unroll
+        for (int rr = 0; rr < RG; ++rr) {
+          float2 Cv[NH], acc = dup(0.f);
+          if (!SUM) pairs_load<NT>(&sc[r0 + rr][n0], Cv);
+#pragma unroll
+          for (int j = 0; j < NH; ++j) {
+            h[j] = fma2(a[rr][j], h[j], ub[rr][j]);
+            if (!SUM) acc = j ? fma2(Cv[j], h[j], acc) : mul2(Cv[j], h[j]);
+          }
+          if (!SUM) ys[rr] = acc.x + acc.y;
+        }
+        if (!SUM) {
+          const int at = fold<RG, LN, 1>(ys, lane);
+#pragma unroll
+          for (int i = 0; i < (RG > LN ? RG / LN : 1); ++i) sy[r0 + at + i][cb] = ys[i];
+        }
       }
     }
     __syncthreads();
@@ -221,15 +218,12 @@ __global__ void __launch_bounds__(128) k_scan_fwd(const P p) {
     }
   }
 
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    if (c0 + cb + i >= rep) continue;
-    const int64_t d = dbase + cb + i;
+  if (on) {
     if (SUM) {
-      states_store<NT>(p.carry + (((int64_t)b * p.nseg + k) * p.D + d) * p.N, n0, p.N, h[i]);
-      if (nl == 0) p.sdelta[((int64_t)b * p.nseg + k) * p.D + d] = dsum[i];
+      states_store<NT>(p.carry + (((int64_t)b * p.nseg + k) * p.D + d) * p.N, n0, p.N, h);
+      if (nl == 0) p.sdelta[((int64_t)b * p.nseg + k) * p.D + d] = dsum;
     } else if (!VAR && p.ht && k == p.nseg - 1) {
-      states_store<NT>(p.ht + ((int64_t)b * p.D + d) * p.N, n0, p.N, h[i]);
+      states_store<NT>(p.ht + ((int64_t)b * p.D + d) * p.N, n0, p.N, h);
     }
   }
   if (SUM && VAR && blockIdx.x == 0 && tid == 0) p.broken[k] = broken != 0;
@@ -309,11 +303,8 @@ __global__ void __launch_bounds__(256) k_scan_step(const P p, int Q, int R) {
   }
 }
 
-// channels of a forward thread: two share the loads of B and C
-int fwd_channels(const P& p) { return (int64_t)blocks_of(p, 128 / lanes_of(p.N) * 2) * p.B >= kFwdBlocks ? 2 : 1; }
-
 size_t plan_fwd(P& p, void* ws) {
-  split(p, blocks_of(p, 128 / lanes_of(p.N)), kFwdBlocks);
+  split(p, blocks_of(p, kFwdThreads / lanes_of(p.N)), kFwdBlocks);
   Carve c{static_cast<char*>(ws)};
   return carve_segments(p, c);
 }
@@ -352,8 +343,8 @@ TOPS_API int tops_gla_ssm_scan_fwd(const tops_gla_scan_args* a, void* stream) {
     LaunchTimer lt(st, "ssm_scan_sum");
     by_shape(p, a->dtype, [&](auto t, auto ln, auto nt, auto var) {
       constexpr int LN = decltype(ln)::value;
-      k_scan_fwd<decltype(t), LN, decltype(nt)::value, 1, decltype(var)::value, true>
-          <<<dim3(blocks_of(p, 128 / LN), p.B, p.nseg - 1), 128, 0, st>>>(p);
+      k_scan_fwd<decltype(t), LN, decltype(nt)::value, decltype(var)::value, true>
+          <<<dim3(blocks_of(p, kFwdThreads / LN), p.B, p.nseg - 1), kFwdThreads, 0, st>>>(p);
       return 0;
     });
     TOPS_CUDA_LAUNCH_CHECK("ssm_scan_sum");
@@ -361,13 +352,10 @@ TOPS_API int tops_gla_ssm_scan_fwd(const tops_gla_scan_args* a, void* stream) {
     TOPS_CUDA_LAUNCH_CHECK("ssm_scan_chain");
   }
   LaunchTimer lt(st, "ssm_scan_fwd");
-  const int ch = p.nseg > 1 ? 1 : fwd_channels(p);
   by_shape(p, a->dtype, [&](auto t, auto ln, auto nt, auto var) {
-    using T = decltype(t);
-    constexpr int LN = decltype(ln)::value, NT = decltype(nt)::value;
-    constexpr bool VAR = decltype(var)::value;
-    if (ch == 2) k_scan_fwd<T, LN, NT, 2, VAR, false><<<dim3(blocks_of(p, 256 / LN), p.B, p.nseg), 128, 0, st>>>(p);
-    else k_scan_fwd<T, LN, NT, 1, VAR, false><<<dim3(blocks_of(p, 128 / LN), p.B, p.nseg), 128, 0, st>>>(p);
+    constexpr int LN = decltype(ln)::value;
+    k_scan_fwd<decltype(t), LN, decltype(nt)::value, decltype(var)::value, false>
+        <<<dim3(blocks_of(p, kFwdThreads / LN), p.B, p.nseg), kFwdThreads, 0, st>>>(p);
     return 0;
   });
   TOPS_CUDA_LAUNCH_CHECK("ssm_scan_fwd");

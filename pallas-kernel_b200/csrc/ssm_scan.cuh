@@ -7,8 +7,8 @@
 //
 // One exponential per (row, channel, state): at N = 16 the exponential unit (16 a clock and SM) bounds the
 // forward at twice the time that its bytes take, and instruction issue the backward.  So:
-//  * a thread owns CH channels x NT states and keeps their states, A and gradients in registers over all
-//    rows; LN lanes share a channel and the other lanes are other channels;
+//  * a thread owns NT states of one channel and keeps them, A and their gradients in registers over all rows; LN
+//    lanes share a channel and the other lanes are other channels;
 //  * what a row needs once per channel (delta, delta x, dy) or once per state (B, C) is computed once per
 //    block, a tile of rows ahead, into shared memory; the tile's elementwise work (softplus, gates,
 //    rounding, 8- or 16-byte accesses) is spread over all threads, its loads issued one tile early;
@@ -27,7 +27,10 @@
 namespace tops {
 namespace ssm {
 
-constexpr int CK = 16;  // rows between saved states = rows of a backward tile
+// Rows between saved states: 4 N / 8 bytes a row and channel, as much as two rows of fp32 at N = 16.  The backward
+// recomputes that many rows of states at a time in registers; with 16 rows between them it had to sweep the first 8
+// twice.
+constexpr int CK = 8;
 
 struct P {
   int B, T, D, N, G, S, softplus;
@@ -55,33 +58,11 @@ struct P {
   float* dh0;
 };
 
-constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
+constexpr float kLn2 = 0.69314718055994531f;
 // ex2.approx errs by -2e-8 on average where decays lie (against 64 bits, arguments -1 .. -0.002), and a state's
 // error is that times the rows it remembers: the exponent's multiply-add takes the mean error back.
 constexpr float kEx2Mean = 2.0e-8f * kLog2e;
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
 // exp(delta A) of a pair, A given times log2(e)
 __device__ __forceinline__ float2 decay2(float delta, float2 A) {
   const float2 e = fma2(dup(delta), A, dup(kEx2Mean));
@@ -228,19 +209,27 @@ __global__ void __launch_bounds__(128) k_scan_chain(const P p) {
   const int b = blockIdx.y;
   if (i >= dn) return;
   const float A = p.A[i] * kLog2e;
+  const int ch = (int)(i / p.N);
   float c = BACK && p.dht && !p.cu ? p.dht[b * dn + i] : 0.f;
-  for (int s = 0; s < p.nseg; ++s) {
-    const int k = BACK ? p.nseg - 1 - s : s;
-    if (s == p.nseg - 1) {
-      p.carry[((int64_t)b * p.nseg + k) * dn + i] = c;
-      break;
+  constexpr int U = 8;  // segments whose loads are in flight together
+  for (int s0 = 0; s0 < p.nseg; s0 += U) {
+    float own[U], decay[U];
+    bool cut[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u, k = BACK ? p.nseg - 1 - s : s;
+      if (s >= p.nseg - 1) continue;  // the last segment passes nothing on
+      own[u] = p.carry[((int64_t)b * p.nseg + k) * dn + i];
+      decay[u] = ex2(A * p.sdelta[((int64_t)b * p.nseg + k) * p.D + ch]);
+      cut[u] = (p.cu && p.broken[k]) || (!BACK && s == 0);  // segment 0 forward began with h0 itself
     }
-    const int64_t at = ((int64_t)b * p.nseg + k) * dn + i;
-    const float own = p.carry[at];
-    p.carry[at] = c;
-    // segment 0 forward began with h0 itself
-    if ((p.cu && p.broken[k]) || (!BACK && s == 0)) c = own;
-    else c = fmaf(ex2(A * p.sdelta[((int64_t)b * p.nseg + k) * p.D + i / p.N]), c, own);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u, k = BACK ? p.nseg - 1 - s : s;
+      if (s >= p.nseg) break;
+      p.carry[((int64_t)b * p.nseg + k) * dn + i] = c;
+      if (s < p.nseg - 1) c = cut[u] ? own[u] : fmaf(decay[u], c, own[u]);
+    }
   }
 }
 
@@ -254,7 +243,10 @@ static __global__ void k_scan_empty(int S, int T, int64_t DN, const int32_t* __r
     to[n * DN + i] = from ? from[n * DN + i] : 0.f;
 }
 
-constexpr int kMinSegment = 128, kFwdBlocks = 148, kBwdBlocks = 148;
+// A block walks its rows alone.  Measured at T = 2048, N = 16 (us, one segment against split): forward blocks of 128
+// threads 128: 148 / 115, 192: 190 / 165, 256: 190 / 220; backward blocks of 256 threads 128: 711 / 530, 192: 960 / 785,
+// 256: 961 / 1046.  So rows are split below 1.5 (1.6) blocks an SM, into enough segments for 8 blocks an SM.
+constexpr int kSms = 148, kFwdBlocks = kSms * 3 / 2, kBwdBlocks = kSms * 8 / 5, kSplitBlocks = kSms * 8, kMinSegment = 64;
 
 inline int check(const tops_gla_scan_args* a) {
   TOPS_CHECK_ARG(a != nullptr, "ssm_scan: args is NULL");
@@ -328,14 +320,12 @@ struct Carve {
   }
 };
 
-// Rows of a segment.  A block walks its rows alone, so without enough blocks the SMs idle; every split costs the
-// exponentials of a first pass.
 inline void split(P& p, int blocks_per_row, int blocks_wanted) {
   p.seg = std::max(p.T, 1);
   p.nseg = 1;
   const int64_t blocks = (int64_t)blocks_per_row * p.B;
   if (blocks >= blocks_wanted || p.T < 2 * kMinSegment) return;
-  const int want = (int)std::min<int64_t>((2 * blocks_wanted + blocks - 1) / blocks, p.T / kMinSegment);
+  const int want = (int)std::min<int64_t>((kSplitBlocks + blocks - 1) / blocks, p.T / kMinSegment);
   if (want < 2) return;
   p.seg = ((p.T + want - 1) / want + 31) / 32 * 32;
   p.nseg = (p.T + p.seg - 1) / p.seg;

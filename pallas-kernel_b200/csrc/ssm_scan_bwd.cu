@@ -4,28 +4,73 @@
 namespace tops {
 namespace ssm {
 
-constexpr int kBwdThreads = 256;
+constexpr int kBwdThreads = 256, kBwdRows = 16, kBwdPart = 4;  // rows of a tile, and of what is in registers at once
+
+// The sums of dB and dC over a warp's channels halve what a lane carries with every exchange.  Which half a lane keeps
+// follows its number; instead of selecting, a lane holds its NT states in an order of its own, register j for state
+// n0 + (j ^ order), so that it always keeps the lower registers.  B and C lie in shared memory in each order, so that a
+// row is still one load.
 template <int LN, int NT>
-constexpr size_t bwd_smem() {
-  return sizeof(float) * CK * ((kBwdThreads / LN) * 6 + 2 * LN * NT + 8 * 2 * LN * NT);
+struct Order {
+  static constexpr int BITS = NT == 2 ? 1 : LN <= 8 ? 2 : 1;  // exchanges that halve the states
+  static constexpr int COPIES = 1 << BITS;
+  static __device__ __forceinline__ int of(int lane) {
+    int o = lane & LN ? NT / 2 : 0;
+    if (BITS == 2 && (lane & (2 * LN))) o |= 1;
+    return o;
+  }
+  // the place of an order's copy: the two orders of a quarter warp lie side by side (no bank conflict)
+  static constexpr __device__ __forceinline__ int slot(int order) {
+    return NT == 2 ? order : BITS == 2 ? (order & 1) << 1 | order >> 1 : order >> 1;
+  }
+  static constexpr __device__ __forceinline__ int order_at(int slot) {
+    return NT == 2 ? slot : BITS == 2 ? (slot & 1) << 1 | slot >> 1 : slot << 1;
+  }
+};
+template <int NT>
+__device__ __forceinline__ void ordered_load(const float* p, int n0, int order, int N, float2 (&h)[NT / 2]) {
+#pragma unroll
+  for (int i = 0; i < NT / 2; ++i) {
+    const int a = n0 + ((2 * i) ^ order), b = n0 + ((2 * i + 1) ^ order);
+    h[i] = make_float2(a < N ? p[a] : 0.f, b < N ? p[b] : 0.f);
+  }
+}
+template <int NT>
+__device__ __forceinline__ void ordered_store(float* p, int n0, int order, int N, const float2 (&h)[NT / 2]) {
+#pragma unroll
+  for (int i = 0; i < NT / 2; ++i) {
+    const int a = n0 + ((2 * i) ^ order), b = n0 + ((2 * i + 1) ^ order);
+    if (a < N) p[a] = h[i].x;
+    if (b < N) p[b] = h[i].y;
+  }
 }
 
-// One segment, tile by tile from its end.  A tile's states are computed again from the saved state before it:
-// its first half once more than its second, so that only 8 rows of states and decays are in registers.
+template <int LN, int NT>
+constexpr size_t bwd_smem() {
+  return sizeof(float) * kBwdRows *
+         ((kBwdThreads / LN) * 6 + 2 * Order<LN, NT>::COPIES * LN * NT + kBwdThreads / 32 * 2 * LN * NT);
+}
+
+// One segment, tile by tile from its end.  The states of 8 rows at a time are computed again from the saved state
+// before them and kept in registers with their decays; what the tile's outputs need of the inputs stays packed as it
+// came (a tile's worth of fp32 copies spilled), the rest is read back from shared memory.
 template <typename T, int LN, int NT, bool VAR>
 __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
-  constexpr int TS = CK, HALF = 8, DB = kBwdThreads / LN, NP = LN * NT, QC = DB / 4, NH = NT / 2;
+  constexpr int TS = kBwdRows, HALF = kBwdPart, DB = kBwdThreads / LN, NP = LN * NT, QC = DB / 4, NH = NT / 2;
   extern __shared__ __align__(16) float smem[];
   float2(*su)[DB] = reinterpret_cast<float2(*)[DB]>(smem);                    // delta, delta x
   float(*sdy)[DB] = reinterpret_cast<float(*)[DB]>(smem + TS * DB * 2);
   float(*sq)[TS][DB] = reinterpret_cast<float(*)[TS][DB]>(smem + TS * DB * 3);  // sum g B, sum A a g h, sum C h
-  float(*sb)[NP] = reinterpret_cast<float(*)[NP]>(smem + TS * DB * 6);
-  float(*sc)[NP] = reinterpret_cast<float(*)[NP]>(smem + TS * DB * 6 + TS * NP);
-  float(*sr)[TS][2 * NP] = reinterpret_cast<float(*)[TS][2 * NP]>(smem + TS * DB * 6 + TS * NP * 2);  // a warp's dB, dC
+  using O = Order<LN, NT>;
+  constexpr int NC = O::COPIES * NP;
+  float(*sb)[NC] = reinterpret_cast<float(*)[NC]>(smem + TS * DB * 6);
+  float(*sc)[NC] = reinterpret_cast<float(*)[NC]>(smem + TS * DB * 6 + TS * NC);
+  float(*sr)[TS][2 * NP] = reinterpret_cast<float(*)[TS][2 * NP]>(smem + TS * DB * 6 + TS * NC * 2);  // a warp's dB, dC
   __shared__ int sflag[TS], sseq[TS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nl = lane % LN, b = blockIdx.y, k = blockIdx.z;
   const int rep = p.D / p.G, nblk = (rep + DB - 1) / DB, grp = blockIdx.x / nblk, blk = blockIdx.x - grp * nblk;
   const int c0 = blk * DB, cb = warp * (32 / LN) + lane / LN, n0 = nl * NT;
+  const int order = O::of(lane), m0 = O::slot(order) * NP + n0;  // its states' order and where its B and C begin
   const int64_t dbase = (int64_t)grp * rep + c0;
   const bool on = c0 + cb < rep;
   const int64_t d = dbase + cb;
@@ -33,32 +78,34 @@ __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
   const int nck = (p.T + CK - 1) / CK;
 
   float2 A[NH], g[NH], dA[NH];
-  states_load<NT>(p.A + d * p.N, n0, on ? p.N : 0, A);
+  ordered_load<NT>(p.A + d * p.N, n0, order, on ? p.N : 0, A);
 #pragma unroll
   for (int j = 0; j < NH; ++j) {
     A[j] = mul2(A[j], dup(kLog2e));
     g[j] = dA[j] = dup(0.f);
   }
   if (on) {
-    if (k < p.nseg - 1) states_load<NT>(p.carry + (((int64_t)b * p.nseg + k) * p.D + d) * p.N, n0, p.N, g);
-    else if (!VAR && p.dht) states_load<NT>(p.dht + ((int64_t)b * p.D + d) * p.N, n0, p.N, g);
+    if (k < p.nseg - 1) ordered_load<NT>(p.carry + (((int64_t)b * p.nseg + k) * p.D + d) * p.N, n0, order, p.N, g);
+    else if (!VAR && p.dht) ordered_load<NT>(p.dht + ((int64_t)b * p.D + d) * p.N, n0, order, p.N, g);
   }
 
   // staging: one quad of channels of one row a thread
   const int qc = tid % QC, qr = tid / QC;
   const int valid = min(max(rep - c0 - qc * 4, 0), 4);
   const int64_t qd = dbase + qc * 4;
-  float bias[4], skip[4], dskip[4], dbias[4];
+  float bias[4], dskip[4], dbias[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     bias[i] = p.bias && i < valid ? p.bias[qd + i] : 0.f;
-    skip[i] = p.skip && i < valid ? p.skip[qd + i] : 0.f;
     dskip[i] = dbias[i] = 0.f;
   }
   constexpr int BQ = TS * NP / 4, BN = (BQ + kBwdThreads - 1) / kBwdThreads;
   Quad<T> xr, dr, zr, gr, br[BN], cr[BN];
   float2 hr[NH];
   int flag = 0, seq = 0;
+  auto saved = [&](int t, float2(&h)[NH]) {  // the state before row t
+    ordered_load<NT>(p.states + (((int64_t)b * nck + t / CK) * p.D + d) * p.N, n0, order, on && t < t_end ? p.N : 0, h);
+  };
   auto fetch = [&](int t0) {
     const int t = t0 + qr;
     const int v = (qr < TS && t < t_end) ? valid : 0;
@@ -73,42 +120,41 @@ __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
       quad_load<T>(static_cast<const T*>(p.bm) + b * p.bs[0] + (t0 + row) * p.bs[1] + grp * p.N + n, p.vb, w, br[j]);
       quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + (t0 + row) * p.cs[1] + grp * p.N + n, p.vc, w, cr[j]);
     }
-    states_load<NT>(p.states + (((int64_t)b * nck + t0 / CK) * p.D + d) * p.N, n0, on ? p.N : 0, hr);
+    saved(t0 + TS - CK, hr);
     if (VAR && tid < TS) flag = t0 + tid < t_end ? row_flags(p, t0 + tid, seq) : 0;
   };
 
   const int last = t_end > t_first ? t_first + (t_end - t_first - 1) / TS * TS : t_first - TS;
   if (last >= t_first) fetch(last);
   for (int t0 = last; t0 >= t_first; t0 -= TS) {
+    bool flagged = false;  // a row of the tile begins or ends a sequence, or belongs to none
     if (VAR) {
       if (tid < TS) {
         sflag[tid] = flag;
         sseq[tid] = seq;
       }
-      __syncthreads();
+      flagged = __syncthreads_or(flag);
     }
     const bool gone = qr >= TS || t0 + qr >= t_end || (VAR && (sflag[qr] & kNone));
-    float xf[4], vf[4], zf[4], gf[4], dl[4], dy[4], zs[4];  // kept for the tile's outputs
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      vf[i] = dr.get(i) + bias[i];
-      vf[i + 1] = dr.get(i + 1) + bias[i + 1];
-      float2 v = make_float2(vf[i], vf[i + 1]);
-      if (p.softplus) v = softplus2(v);
-      dl[i] = gone ? 0.f : v.x;
-      dl[i + 1] = gone ? 0.f : v.y;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      xf[i] = gone ? 0.f : xr.get(i);
-      gf[i] = gone ? 0.f : gr.get(i);
-      zf[i] = gone ? 0.f : zr.get(i);
-      zs[i] = fast_sigmoid(zf[i]);
-      dy[i] = p.z ? gf[i] * zf[i] * zs[i] : gf[i];
-    }
+    const Quad<T> xc = xr, dc = dr, zc = zr, gc = gr;  // for the tile's outputs
     if (qr < TS) {
-      *reinterpret_cast<float4*>(&su[qr][qc * 4]) = make_float4(dl[0], dl[0] * xf[0], dl[1], dl[1] * xf[1]);
-      *reinterpret_cast<float4*>(&su[qr][qc * 4 + 2]) = make_float4(dl[2], dl[2] * xf[2], dl[3], dl[3] * xf[3]);
+      float dl[4], dy[4];
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        float2 v = make_float2(dc.get(i) + bias[i], dc.get(i + 1) + bias[i + 1]);
+        if (p.softplus) v = softplus2(v);
+        dl[i] = gone ? 0.f : v.x;
+        dl[i + 1] = gone ? 0.f : v.y;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float z = zc.get(i);
+        dy[i] = gone ? 0.f : p.z ? gc.get(i) * z * fast_sigmoid(z) : gc.get(i);
+      }
+      const float x0 = gone ? 0.f : xc.get(0), x1 = gone ? 0.f : xc.get(1), x2 = gone ? 0.f : xc.get(2),
+                  x3 = gone ? 0.f : xc.get(3);
+      *reinterpret_cast<float4*>(&su[qr][qc * 4]) = make_float4(dl[0], dl[0] * x0, dl[1], dl[1] * x1);
+      *reinterpret_cast<float4*>(&su[qr][qc * 4 + 2]) = make_float4(dl[2], dl[2] * x2, dl[3], dl[3] * x3);
       *reinterpret_cast<float4*>(&sdy[qr][qc * 4]) = make_float4(dy[0], dy[1], dy[2], dy[3]);
     }
 #pragma unroll
@@ -122,126 +168,173 @@ __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
           fb[i] = none ? 0.f : br[j].get(i);
           fc[i] = none ? 0.f : cr[j].get(i);
         }
-        *reinterpret_cast<float4*>(&sb[row][n]) = make_float4(fb[0], fb[1], fb[2], fb[3]);
-        *reinterpret_cast<float4*>(&sc[row][n]) = make_float4(fc[0], fc[1], fc[2], fc[3]);
+#pragma unroll
+        for (int c = 0; c < O::COPIES; ++c) {
+          const int o = O::order_at(c);
+          *reinterpret_cast<float4*>(&sb[row][c * NP + n]) = make_float4(fb[o], fb[1 ^ o], fb[2 ^ o], fb[3 ^ o]);
+          *reinterpret_cast<float4*>(&sc[row][c * NP + n]) = make_float4(fc[o], fc[1 ^ o], fc[2 ^ o], fc[3 ^ o]);
+        }
       }
     }
-    float2 hs[NH];
+    float2 h[NH], hc[NH], hs[NH];  // the state, the saved one of this part, and of the part before it
 #pragma unroll
-    for (int j = 0; j < NH; ++j) hs[j] = hr[j];
+    for (int j = 0; j < NH; ++j) hc[j] = hr[j];
     __syncthreads();
     if (t0 > t_first) fetch(t0 - TS);
 
-    // the state before row r (a sequence's first row starts anew)
-    auto enter = [&](int r, float2(&h)[NH]) {
-      if (VAR && (sflag[r] & (kFirst | kNone))) {
+    auto rows = [&](auto with_flags) {
+      constexpr bool FLAG = decltype(with_flags)::value;
+      // the state before row r (a sequence's first row starts anew)
+      auto enter = [&](int r, float2(&h)[NH]) {
+        if (FLAG && (sflag[r] & (kFirst | kNone))) {
 #pragma unroll
-        for (int j = 0; j < NH; ++j) h[j] = dup(0.f);
-        if ((sflag[r] & kFirst) && p.h0 && on) states_load<NT>(p.h0 + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, h);
-      }
-    };
+          for (int j = 0; j < NH; ++j) h[j] = dup(0.f);
+          if ((sflag[r] & kFirst) && p.h0 && on) ordered_load<NT>(p.h0 + ((int64_t)sseq[r] * p.D + d) * p.N, n0, order, p.N, h);
+        }
+      };
 #pragma unroll 1
-    for (int half = 1; half >= 0; --half) {
-      float2 h[NH];
+      for (int part = TS / HALF - 1; part >= 0; --part) {
+        const int r0 = part * HALF;
+        if (HALF == CK || part % (CK / HALF) == CK / HALF - 1) {  // a new saved state; the one before it is on its way
+          if (part != TS / HALF - 1)
 #pragma unroll
-      for (int j = 0; j < NH; ++j) h[j] = hs[j];
-      if (half == 1) {
+            for (int j = 0; j < NH; ++j) hc[j] = hs[j];
+          if (r0 - (CK - HALF) >= CK) saved(t0 + r0 - (CK - HALF) - CK, hs);
+        }
+#pragma unroll
+        for (int j = 0; j < NH; ++j) h[j] = hc[j];
+        if (HALF < CK && part % (CK / HALF) != 0) {
+#pragma unroll
+          for (int rr = 0; rr < CK - HALF; ++rr) {
+            const int r = r0 - (CK - HALF) + rr;
+            enter(r, h);
+            float2 Bv[NH];
+            pairs_load<NT>(&sb[r][m0], Bv);
+            const float2 q = su[r][cb];
+#pragma unroll
+            for (int j = 0; j < NH; ++j) h[j] = fma2(decay2(q.x, A[j]), h[j], mul2(dup(q.y), Bv[j]));
+          }
+        }
+        float2 a[HALF][NH], hp[HALF + 1][NH];
 #pragma unroll
         for (int r = 0; r < HALF; ++r) {
-          enter(r, h);
+          enter(r0 + r, h);
           float2 Bv[NH];
-          pairs_load<NT>(&sb[r][n0], Bv);
-          const float2 q = su[r][cb];
-#pragma unroll
-          for (int j = 0; j < NH; ++j) h[j] = fma2(decay2(q.x, A[j]), h[j], mul2(dup(q.y), Bv[j]));
-        }
-      }
-      const int r0 = half * HALF;
-      float2 a[HALF][NH], hp[HALF + 1][NH];
-#pragma unroll
-      for (int r = 0; r < HALF; ++r) {
-        enter(r0 + r, h);
-        float2 Bv[NH];
-        pairs_load<NT>(&sb[r0 + r][n0], Bv);
-        const float2 q = su[r0 + r][cb];
-#pragma unroll
-        for (int j = 0; j < NH; ++j) {
-          hp[r][j] = h[j];
-          a[r][j] = decay2(q.x, A[j]);
-          h[j] = fma2(a[r][j], h[j], mul2(dup(q.y), Bv[j]));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NH; ++j) hp[HALF][j] = h[j];
-#pragma unroll
-      for (int r4 = HALF - 4; r4 >= 0; r4 -= 4) {
-        float s1[4], s2[4], s3[4];
-#pragma unroll
-        for (int rr = 3; rr >= 0; --rr) {
-          const int r = r4 + rr;
-          if (VAR && (sflag[r0 + r] & (kLast | kNone))) {
-#pragma unroll
-            for (int j = 0; j < NH; ++j) g[j] = dup(0.f);
-            if ((sflag[r0 + r] & kLast) && p.dht && on)
-              states_load<NT>(p.dht + ((int64_t)sseq[r0 + r] * p.D + d) * p.N, n0, p.N, g);
-          }
-          float2 Bv[NH], Cv[NH], w1 = dup(0.f), w2 = dup(0.f), w3 = dup(0.f);
-          pairs_load<NT>(&sb[r0 + r][n0], Bv);
-          pairs_load<NT>(&sc[r0 + r][n0], Cv);
+          pairs_load<NT>(&sb[r0 + r][m0], Bv);
           const float2 q = su[r0 + r][cb];
-          const float dyv = sdy[r0 + r][cb];
-          float bc[2 * NT];
 #pragma unroll
           for (int j = 0; j < NH; ++j) {
-            float2 ht = hp[r + 1][j];
-            if (VAR) ht = fma2(a[r][j], hp[r][j], mul2(dup(q.y), Bv[j]));  // the next row may have started anew
-            g[j] = fma2(Cv[j], dup(dyv), g[j]);
-            w1 = j ? fma2(g[j], Bv[j], w1) : mul2(g[j], Bv[j]);
-            w3 = j ? fma2(Cv[j], ht, w3) : mul2(Cv[j], ht);
-            const float2 vb = mul2(g[j], dup(q.y)), vc = mul2(ht, dup(dyv));
-            bc[2 * j] = vb.x; bc[2 * j + 1] = vb.y;
-            bc[NT + 2 * j] = vc.x; bc[NT + 2 * j + 1] = vc.y;
-            g[j] = mul2(a[r][j], g[j]);
-            const float2 w = mul2(g[j], hp[r][j]);
-            w2 = j ? fma2(A[j], w, w2) : mul2(A[j], w);
-            dA[j] = fma2(dup(q.x), w, dA[j]);
+            hp[r][j] = h[j];
+            a[r][j] = decay2(q.x, A[j]);
+            h[j] = fma2(a[r][j], h[j], mul2(dup(q.y), Bv[j]));
           }
-          s1[rr] = w1.x + w1.y;
-          s2[rr] = w2.x + w2.y;
-          s3[rr] = w3.x + w3.y;
-          const int at = fold<2 * NT, 32 / LN, LN>(bc, lane);  // over the warp's channels
-          constexpr int KEEP = 2 * NT / (32 / LN) > 1 ? 2 * NT / (32 / LN) : 1;
-#pragma unroll
-          for (int i = 0; i < KEEP; ++i)
-            sr[warp][r0 + r][((at + i) / NT) * NP + n0 + (at + i) % NT] = bc[i];
-          if (VAR && (sflag[r0 + r] & kFirst) && p.dh0 && on)
-            states_store<NT>(p.dh0 + ((int64_t)sseq[r0 + r] * p.D + d) * p.N, n0, p.N, g);
         }
-        const int o1 = fold<4, LN, 1>(s1, lane);  // over the lanes of a channel
-        fold<4, LN, 1>(s2, lane);
-        fold<4, LN, 1>(s3, lane);
-        sq[0][r0 + r4 + o1][cb] = s1[0];
-        sq[1][r0 + r4 + o1][cb] = s2[0];
-        sq[2][r0 + r4 + o1][cb] = s3[0];
+#pragma unroll
+        for (int j = 0; j < NH; ++j) hp[HALF][j] = h[j];
+#pragma unroll
+        for (int r4 = HALF - 4; r4 >= 0; r4 -= 4) {
+          float s1[4], s2[4], s3[4];
+#pragma unroll
+          for (int rr = 3; rr >= 0; --rr) {
+            const int r = r4 + rr;
+            if (FLAG && (sflag[r0 + r] & (kLast | kNone))) {
+#pragma unroll
+              for (int j = 0; j < NH; ++j) g[j] = dup(0.f);
+              if ((sflag[r0 + r] & kLast) && p.dht && on)
+                ordered_load<NT>(p.dht + ((int64_t)sseq[r0 + r] * p.D + d) * p.N, n0, order, p.N, g);
+            }
+            float2 Bv[NH], Cv[NH], w1 = dup(0.f), w2 = dup(0.f), w3 = dup(0.f);
+            pairs_load<NT>(&sb[r0 + r][m0], Bv);
+            pairs_load<NT>(&sc[r0 + r][m0], Cv);
+            const float2 q = su[r0 + r][cb];
+            const float dyv = sdy[r0 + r][cb];
+            float vb[NT], vc[NT];  // terms of dB and dC
+#pragma unroll
+            for (int j = 0; j < NH; ++j) {
+              float2 ht = hp[r + 1][j];
+              if (FLAG) ht = fma2(a[r][j], hp[r][j], mul2(dup(q.y), Bv[j]));  // the next row may have started anew
+              g[j] = fma2(Cv[j], dup(dyv), g[j]);
+              w1 = j ? fma2(g[j], Bv[j], w1) : mul2(g[j], Bv[j]);
+              w3 = j ? fma2(Cv[j], ht, w3) : mul2(Cv[j], ht);
+              const float2 tb = mul2(g[j], dup(q.y)), tc = mul2(ht, dup(dyv));
+              vb[2 * j] = tb.x; vb[2 * j + 1] = tb.y;
+              vc[2 * j] = tc.x; vc[2 * j + 1] = tc.y;
+              g[j] = mul2(a[r][j], g[j]);
+              const float2 w = mul2(g[j], hp[r][j]);
+              w2 = j ? fma2(A[j], w, w2) : mul2(A[j], w);
+              dA[j] = fma2(dup(q.x), w, dA[j]);
+            }
+            s1[rr] = w1.x + w1.y;
+            s2[rr] = w2.x + w2.y;
+            s3[rr] = w3.x + w3.y;
+            // over the warp's channels: first the states are halved, then one of dB and dC is kept, then nothing is left to halve
+            constexpr int KEEP = NT >> O::BITS;
+            int m = LN;
+#pragma unroll
+            for (int i = 0; i < O::BITS; ++i, m <<= 1)
+#pragma unroll
+              for (int j = 0; j < (NT >> (i + 1)); ++j) {
+                vb[j] += __shfl_xor_sync(0xffffffffu, vb[j + (NT >> (i + 1))], m);
+                vc[j] += __shfl_xor_sync(0xffffffffu, vc[j + (NT >> (i + 1))], m);
+              }
+            float* out = &sr[warp][r0 + r][n0];
+            if constexpr ((LN << O::BITS) < 32) {
+              const bool up = lane & (LN << O::BITS);
+              float keep = up ? vc[0] : vb[0];
+              keep += __shfl_xor_sync(0xffffffffu, up ? vb[0] : vc[0], LN << O::BITS);
+#pragma unroll
+              for (int mm = LN << (O::BITS + 1); mm < 32; mm <<= 1) keep += __shfl_xor_sync(0xffffffffu, keep, mm);
+              out[(up ? NP : 0) + order] = keep;
+            } else {
+#pragma unroll
+              for (int j = 0; j < KEEP; ++j) {
+                out[j ^ order] = vb[j];
+                out[NP + (j ^ order)] = vc[j];
+              }
+            }
+            if (FLAG && (sflag[r0 + r] & kFirst) && p.dh0 && on)
+              ordered_store<NT>(p.dh0 + ((int64_t)sseq[r0 + r] * p.D + d) * p.N, n0, order, p.N, g);
+          }
+          const int o1 = fold<4, LN, 1>(s1, lane);  // over the lanes of a channel
+          fold<4, LN, 1>(s2, lane);
+          fold<4, LN, 1>(s3, lane);
+          sq[0][r0 + r4 + o1][cb] = s1[0];
+          sq[1][r0 + r4 + o1][cb] = s2[0];
+          sq[2][r0 + r4 + o1][cb] = s3[0];
+        }
       }
-    }
+    };
+    if (VAR && flagged) rows(std::true_type());
+    else rows(std::false_type());
     __syncthreads();
 
     const int t = t0 + qr;
     if (qr < TS && t < t_end) {
       const bool none = VAR && (sflag[qr] & kNone);
-      float odx[4], oddt[4], odz[4];
+      float odx[4], oddt[4], odz[4], sk[4];
+      const float4 u0 = *reinterpret_cast<const float4*>(&su[qr][qc * 4]);
+      const float4 u1 = *reinterpret_cast<const float4*>(&su[qr][qc * 4 + 2]);
+      const float4 dy4 = *reinterpret_cast<const float4*>(&sdy[qr][qc * 4]);
+      const float4 q0 = *reinterpret_cast<const float4*>(&sq[0][qr][qc * 4]);
+      const float4 q1 = *reinterpret_cast<const float4*>(&sq[1][qr][qc * 4]);
+      const float4 q2 = *reinterpret_cast<const float4*>(&sq[2][qr][qc * 4]);
+      const float dl[4] = {u0.x, u0.z, u1.x, u1.z}, dy[4] = {dy4.x, dy4.y, dy4.z, dy4.w};
+      const float gB[4] = {q0.x, q0.y, q0.z, q0.w}, aw[4] = {q1.x, q1.y, q1.z, q1.w}, ch[4] = {q2.x, q2.y, q2.z, q2.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sk[i] = p.skip && i < valid ? p.skip[qd + i] : 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float gB = sq[0][qr][qc * 4 + i], aw = sq[1][qr][qc * 4 + i] * kLn2;
-        const float y = fmaf(skip[i], xf[i], sq[2][qr][qc * 4 + i]);
-        odx[i] = none ? 0.f : fmaf(dl[i], gB, skip[i] * dy[i]);
-        float dv = fmaf(xf[i], gB, aw);
-        if (p.softplus) dv *= fast_sigmoid(vf[i]);
+        const float x = xc.get(i);
+        odx[i] = none ? 0.f : fmaf(dl[i], gB[i], sk[i] * dy[i]);
+        float dv = fmaf(x, gB[i], aw[i] * kLn2);
+        if (p.softplus) dv *= fast_sigmoid(dc.get(i) + bias[i]);
         oddt[i] = none ? 0.f : dv;
-        odz[i] = none ? 0.f : gf[i] * y * zs[i] * fmaf(zf[i], 1.f - zs[i], 1.f);
         dbias[i] += oddt[i];
-        dskip[i] = fmaf(dy[i], xf[i], dskip[i]);
+        dskip[i] = none ? dskip[i] : fmaf(dy[i], x, dskip[i]);
+        if (p.dz) {
+          const float z = zc.get(i), zs = fast_sigmoid(z), y = fmaf(sk[i], x, ch[i]);
+          odz[i] = none ? 0.f : gc.get(i) * y * zs * fmaf(z, 1.f - zs, 1.f);
+        }
       }
       const int64_t o = ((int64_t)b * p.T + t) * p.D + qd;
       quad_store<T>(static_cast<T*>(p.dx) + o, p.vg, valid, odx);
@@ -263,8 +356,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
 
   const int64_t sg = (int64_t)b * p.nseg + k;
   if (on) {
-    states_store<NT>(p.pa + (sg * p.D + d) * p.N, n0, p.N, dA);
-    if (!VAR && p.dh0 && k == 0) states_store<NT>(p.dh0 + ((int64_t)b * p.D + d) * p.N, n0, p.N, g);
+    ordered_store<NT>(p.pa + (sg * p.D + d) * p.N, n0, order, p.N, dA);
+    if (!VAR && p.dh0 && k == 0) ordered_store<NT>(p.dh0 + ((int64_t)b * p.D + d) * p.N, n0, order, p.N, g);
   }
   // dD and dbias: the rows' threads of a quad, in a fixed order
   __syncthreads();
@@ -472,7 +565,7 @@ TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream
       constexpr int LN = decltype(ln)::value, NT = decltype(nt)::value;
       auto kernel = k_scan_bwd<decltype(t), LN, NT, decltype(var)::value>;
       constexpr size_t bytes = bwd_smem<LN, NT>();
-      if (bytes > 48 * 1024) {
+      if (bytes > 47 * 1024) {  // the rows' flags come on top
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != cudaSuccess) return cuda_status(e, "ssm_scan_bwd");
       }
@@ -497,9 +590,9 @@ TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream
       {p.D, 2 * (int64_t)p.D, p.pd + p.D, a->ddt_bias}};
   for (const auto& s : sums) {
     if (!s.out) continue;
-    LaunchTimer lt(st, "ssm_scan_sum");
+    LaunchTimer lt(st, "ssm_scan_param");
     k_scan_sum<<<(unsigned)((s.n + 255) / 256), 256, 0, st>>>(p.B * p.nseg, s.n, s.stride, s.part, s.out);
-    TOPS_CUDA_LAUNCH_CHECK("ssm_scan_sum");
+    TOPS_CUDA_LAUNCH_CHECK("ssm_scan_param");
   }
   return TOPS_OK;
 }
