@@ -75,18 +75,6 @@ __device__ __forceinline__ void load_params(const P& p, int d0, float (&w)[W][V]
 // that several batches of R rows are in flight without registers and no thread waits for another.
 constexpr int R = 4;
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-  const uint32_t a = (uint32_t)__cvta_generic_to_shared(dst);
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(a), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int AHEAD>
-__device__ __forceinline__ void copies_wait() {  // all but the last AHEAD groups have arrived
-  asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
-}
-
 // the sequence of row t of batch row b: [s, e) and its number (-1: none)
 __device__ __forceinline__ SeqAt seq_of(const P& p, int b, int t) {
   if (p.cu == nullptr) return SeqAt{b, 0, p.T};

@@ -5,10 +5,9 @@
 // Backward: dn = the rotation by the opposite angle of dy, e = w dn, dw = sum dn x s,
 //   dx = s (e - x s^2 mean(e x)).
 //
-// Nothing is reused between rows but the token's cosines and the weights, so HBM bounds it:
-// a group of lanes owns a token, keeps V weights a lane in registers and walks the token's heads.
-// A rotated element's partner lies in another lane's vector: it is loaded once more (the line is
-// in L1) rather than passed through shuffles whose register index would be dynamic.
+// Nothing is reused between rows but the token's cosines and the weights, so HBM bounds it: a group of lanes owns a
+// token and walks its heads, V elements a lane.  The heads' vectors come through a ring in shared memory, several heads
+// ahead of their use and without registers; a rotated element's partner is read there from the other lane's column.
 #include <algorithm>
 
 #include "rowtypes.cuh"
@@ -20,8 +19,8 @@ struct P {
   int64_t tokens;
   int T, H, HK, K, R, pairs, wdtype, pos64, table;
   int lanes, hg, nhg;  // lanes of a row, heads of a unit, units of a token
-  int wvec;            // the weights start on a vector
-  float eps;
+  int wvec, tvec;      // the weights and the tables start on a vector
+  float eps, inv_k;
   const void *q, *k, *qw, *kw;
   int64_t qs[3], ks[3];  // strides (batch, row, head) of q and k in elements
   const float *cos, *sin;
@@ -39,7 +38,7 @@ struct P {
 // cosine and signed sine (y_i = n_i c_i + n_partner s_i).
 template <int V>
 struct Rot {
-  int p0;  // first partner's element (half-split); interleaved partners are inside the vector
+  int p0;  // first partner's element (half-split); interleaved partners are inside the vector (V > 1)
   bool on;
   float c[V], s[V];
 };
@@ -72,10 +71,21 @@ __device__ __forceinline__ Rot<V> rotation(const P& p, int e0, int64_t pos, floa
     const bool low = e0 < half;
     const int a = low ? e0 : e0 - half;
     r.p0 = low ? e0 + half : e0 - half;
+    float c[V], s[V];
+    if (p.tvec) {  // half is a multiple of V
+      Vx<float, V>::load(ct + a, c);
+      Vx<float, V>::load(st + a, s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        c[i] = ct[a + i];
+        s[i] = st[a + i];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      r.c[i] = inside ? ct[a + i] : bad;
-      r.s[i] = inside ? (low ? -sign : sign) * st[a + i] : bad;
+      r.c[i] = inside ? c[i] : bad;
+      r.s[i] = inside ? (low ? -sign : sign) * s[i] : bad;
     }
   }
   return r;
@@ -97,198 +107,165 @@ __device__ __forceinline__ void weights(const void* w, const P& p, int e0, float
   }
 }
 
-// The heads h0 .. h1 of q (or of k) of one token, HB at a time: their loads are issued before the first sum.
-// Every lane of a warp takes the same turns, since the sums are full-warp exchanges; `live` says whose rows exist.
-template <typename T, int V, int J, int HB>
-__device__ __forceinline__ void heads_fwd(const P& p, const T* x, int64_t hs, T* y, const void* weight, int h0, int h1,
-                                          int turns, bool live, int l, const Rot<V> (&rot)[J]) {
-  float w[J][V], pw[J][V];
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    weights<T, V>(weight, p, (l + j * p.lanes) * V, w[j]);
-    weights<T, V>(weight, p, rot[j].p0, pw[j]);
-  }
-  for (int i = 0; i < turns; i += HB) {
-    Raw<T, V> own[HB][J], par[HB][J];
-#pragma unroll
-    for (int u = 0; u < HB; ++u)
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int e0 = (l + j * p.lanes) * V;
-        if (live && h0 + i + u < h1 && e0 < p.K) {
-          own[u][j].load(x + (h0 + i + u) * hs + e0);
-          if (rot[j].on && !(p.pairs && V > 1)) par[u][j].load(x + (h0 + i + u) * hs + rot[j].p0);
-        }
-      }
-    float ss[HB];
-#pragma unroll
-    for (int u = 0; u < HB; ++u) {
-      ss[u] = 0.f;
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        if (live && h0 + i + u < h1 && (l + j * p.lanes) * V < p.K) {
-          float v[V];
-          own[u][j].get(v);
-#pragma unroll
-          for (int c = 0; c < V; ++c) ss[u] = fmaf(v[c], v[c], ss[u]);
-        }
-      }
-    }
-    for (int o = p.lanes >> 1; o > 0; o >>= 1)
-#pragma unroll
-      for (int u = 0; u < HB; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
-#pragma unroll
-    for (int u = 0; u < HB; ++u) {
-      const float s = rsqrtf(ss[u] / (float)p.K + p.eps);
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int e0 = (l + j * p.lanes) * V;
-        if (live && h0 + i + u < h1 && e0 < p.K) {
-          float out[V];
-          own[u][j].get(out);
-#pragma unroll
-          for (int c = 0; c < V; ++c) out[c] *= s * w[j][c];
-          if (rot[j].on) {
-            float o[V];
-            if (p.pairs && V > 1) {
-#pragma unroll
-              for (int c = 0; c < V; ++c) o[c] = out[c ^ (V > 1 ? 1 : 0)];
-            } else {
-              par[u][j].get(o);
-#pragma unroll
-              for (int c = 0; c < V; ++c) o[c] *= s * pw[j][c];
-            }
-#pragma unroll
-            for (int c = 0; c < V; ++c) out[c] = fmaf(out[c], rot[j].c[c], o[c] * rot[j].s[c]);
-          }
-          Vx<T, V>::store(y + (h0 + i + u) * p.K + e0, out);
-        }
-      }
-    }
-  }
-}
-
 __device__ __forceinline__ int64_t position(const P& p, int b, int t) {
   if (!p.R || !p.pos) return t;
   return p.pos64 ? static_cast<const int64_t*>(p.pos)[b * p.pb + t] : static_cast<const int32_t*>(p.pos)[b * p.pb + t];
 }
 
+// A ring of head vectors: kThreads columns of J vectors for each of kSlots heads and each of M tensors.
+constexpr int kThreads = 128, kAhead = 3, kSlots = kAhead + 1, kWarps = kThreads / 32;
+template <typename T, int V, int J, int M>
+struct Ring {
+  Raw<T, V> v[kSlots][M][J][kThreads];
+};
+
+// The heads of a unit, one a turn: every lane of a warp takes every turn, since the sums are full-warp exchanges.  A walk
+// goes over the heads of q, then of k, in one tensor (pointers, no products in the loop).
+template <typename T>
+struct Walk {
+  const T *at, *k;
+  int64_t qs, ks;
+  int h;  // head of q, then of k behind them
+  __device__ __forceinline__ Walk(const P& p, const void* q_, const int64_t (&sq)[3], const void* k_, const int64_t (&sk)[3],
+                                  int b, int t, int h0)
+      : k(static_cast<const T*>(k_) + b * sk[0] + t * sk[1]), qs(sq[2]), ks(sk[2]), h(h0) {
+    at = h0 < p.H ? static_cast<const T*>(q_) + b * sq[0] + t * sq[1] + h0 * qs : k + (h0 - p.H) * ks;
+  }
+  __device__ __forceinline__ void next(const P& p) {
+    at += h < p.H ? qs : ks;
+    if (++h == p.H) at = k;
+  }
+};
+template <typename T>
+struct Out {
+  T *at, *k;
+  int h;
+  __device__ __forceinline__ Out(const P& p, void* q_, void* k_, int64_t tok, int h0)
+      : k(static_cast<T*>(k_) + tok * p.HK * p.K), h(h0) {
+    at = h0 < p.H ? static_cast<T*>(q_) + (tok * p.H + h0) * p.K : k + (h0 - p.H) * p.K;
+  }
+  __device__ __forceinline__ void next(const P& p) {
+    at += p.K;
+    if (++h == p.H) at = k;
+  }
+};
+__device__ __forceinline__ float group_sum(float v, int lanes) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {  // selected, not branched over: the branch would cost a convergence each
+    const float r = __shfl_xor_sync(0xffffffffu, v, o);
+    v += lanes > o ? r : 0.f;
+  }
+  return v;
+}
+
 template <typename T, int V, int J>
-__global__ void __launch_bounds__(256) k_qk_fwd(const P p) {
-  constexpr int HB = J == 1 ? 4 : 1;
-  const int lane = threadIdx.x & 31, l = lane & (p.lanes - 1);
+__global__ void __launch_bounds__(kThreads) k_qk_fwd(const P p) {
+  __shared__ Ring<T, V, J, 1> ring;
+  const int tid = threadIdx.x, lane = tid & 31, l = lane & (p.lanes - 1), base = tid - l;
   const int rpw = 32 / p.lanes;
-  const int64_t unit = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * rpw + lane / p.lanes;
+  const int64_t unit = ((int64_t)blockIdx.x * kWarps + (tid >> 5)) * rpw + lane / p.lanes;
   const bool live = unit < p.tokens * p.nhg;
   const int64_t tok = live ? unit / p.nhg : 0;
-  const int h0 = live ? (int)(unit - tok * p.nhg) * p.hg : 0, h1 = h0 + p.hg;
+  const int h0 = live ? (int)(unit - tok * p.nhg) * p.hg : 0;
   const int b = (int)(tok / p.T), t = (int)(tok - (int64_t)b * p.T);
+  const int turns = live ? min(p.hg, p.H + p.HK - h0) : 0;
+  Walk<T> in(p, p.q, p.qs, p.k, p.ks, b, t, h0);
+  Out<T> out_at(p, p.yq, p.yk, tok, h0);
+  auto ask = [&](int i) {
+    if (i < turns) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int e0 = (l + j * p.lanes) * V;
+        if (e0 < p.K) {
+          Raw<T, V>& to = ring.v[i % kSlots][0][j][tid];
+          if constexpr (V == 1) to.load(in.at + e0);
+          else copy_async<Raw<T, V>::B>(&to, in.at + e0);
+        }
+      }
+      in.next(p);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) ask(i);
   const int64_t pos = position(p, b, t);
   Rot<V> rot[J];
+  float w[J][V], pw[J][V];  // the weight times the cosine, and the partner's times the sine
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int e0 = (l + j * p.lanes) * V;
     rot[j] = rotation<V>(p, e0 < p.K ? e0 : p.K, pos, 1.f);
   }
-  // units of a warp may lie on both sides of the border between q and k: each side's turns are the warp's most
-  const int q1 = min(h1, p.H), k0 = max(h0, p.H) - p.H, k1 = min(h1, p.H + p.HK) - p.H;
-  const int qn = __reduce_max_sync(0xffffffffu, live ? max(q1 - h0, 0) : 0);
-  const int kn = __reduce_max_sync(0xffffffffu, live ? max(k1 - k0, 0) : 0);
-  if (qn > 0)
-    heads_fwd<T, V, J, HB>(p, static_cast<const T*>(p.q) + b * p.qs[0] + t * p.qs[1], p.qs[2],
-                           static_cast<T*>(p.yq) + tok * p.H * p.K, p.qw, h0, q1, qn, live, l, rot);
-  if (kn > 0)
-    heads_fwd<T, V, J, HB>(p, static_cast<const T*>(p.k) + b * p.ks[0] + t * p.ks[1], p.ks[2],
-                           static_cast<T*>(p.yk) + tok * p.HK * p.K, p.kw, k0, k1, kn, live, l, rot);
-}
-
-// As heads_fwd: both sums of a row (x^2 and e x) come from the same loads; the rows' dw terms are kept.
-template <typename T, int V, int J, int HB>
-__device__ __forceinline__ void heads_bwd(const P& p, const T* x, int64_t hs, const T* dy, int64_t gs, T* dx,
-                                          const void* weight, int h0, int h1, int turns, bool live, int l,
-                                          const Rot<V> (&rot)[J], float (&dw)[J][V]) {
-  float w[J][V];
-#pragma unroll
-  for (int j = 0; j < J; ++j) weights<T, V>(weight, p, (l + j * p.lanes) * V, w[j]);
-  for (int i = 0; i < turns; i += HB) {
-    Raw<T, V> xr[HB][J], gr[HB][J], pr[HB][J];
-#pragma unroll
-    for (int u = 0; u < HB; ++u)
+  int of = -1;  // whose weights they are
+  for (int i = 0; i < p.hg; ++i) {
+    copies_wait<kAhead - 1>();
+    __syncwarp();  // the other lanes' copies too, and nobody reads the slot that is filled next
+    ask(i + kAhead);
+    const bool on = i < turns, isq = out_at.h < p.H;
+    if (of != (int)isq) {
+      of = isq;
+      const void* wt = isq ? p.qw : p.kw;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const int e0 = (l + j * p.lanes) * V;
-        if (live && h0 + i + u < h1 && e0 < p.K) {
-          xr[u][j].load(x + (h0 + i + u) * hs + e0);
-          gr[u][j].load(dy + (h0 + i + u) * gs + e0);
-          if (rot[j].on && !(p.pairs && V > 1)) pr[u][j].load(dy + (h0 + i + u) * gs + rot[j].p0);
+        weights<T, V>(wt, p, (l + j * p.lanes) * V, w[j]);
+        if (p.pairs && V > 1) {
+#pragma unroll
+          for (int c = 0; c < V; ++c) pw[j][c] = w[j][c ^ (V > 1 ? 1 : 0)];
+        } else {
+          weights<T, V>(wt, p, rot[j].p0, pw[j]);
         }
-      }
-    float ss[HB], ex[HB];
-    float e[HB][J][V];
-#pragma unroll
-    for (int u = 0; u < HB; ++u) {
-      ss[u] = ex[u] = 0.f;
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        if (live && h0 + i + u < h1 && (l + j * p.lanes) * V < p.K) {
-          float v[V];
-          xr[u][j].get(v);
-          gr[u][j].get(e[u][j]);
-          if (rot[j].on) {
-            float o[V];
-            if (p.pairs && V > 1) {
-#pragma unroll
-              for (int c = 0; c < V; ++c) o[c] = e[u][j][c ^ (V > 1 ? 1 : 0)];
-            } else {
-              pr[u][j].get(o);
-            }
-#pragma unroll
-            for (int c = 0; c < V; ++c) e[u][j][c] = fmaf(e[u][j][c], rot[j].c[c], o[c] * rot[j].s[c]);
-          }
-#pragma unroll
-          for (int c = 0; c < V; ++c) {
-            ss[u] = fmaf(v[c], v[c], ss[u]);
-            ex[u] = fmaf(e[u][j][c] * w[j][c], v[c], ex[u]);
-          }
-        }
+        mul_n<V>(w[j], w[j], rot[j].c);
+        mul_n<V>(pw[j], pw[j], rot[j].s);
       }
     }
-    for (int o = p.lanes >> 1; o > 0; o >>= 1)
+    float v[J][V], ss = 0.f;
 #pragma unroll
-      for (int u = 0; u < HB; ++u) {
-        ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
-        ex[u] += __shfl_xor_sync(0xffffffffu, ex[u], o);
-      }
+    for (int j = 0; j < J; ++j) {
 #pragma unroll
-    for (int u = 0; u < HB; ++u) {
-      const float s = rsqrtf(ss[u] / (float)p.K + p.eps);
-      const float m = s * s * ex[u] / (float)p.K;
+      for (int c = 0; c < V; ++c) v[j][c] = 0.f;
+      if (on && (l + j * p.lanes) * V < p.K) ring.v[i % kSlots][0][j][tid].get(v[j]);
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int e0 = (l + j * p.lanes) * V;
-        if (live && h0 + i + u < h1 && e0 < p.K) {
-          float v[V], out[V];
-          xr[u][j].get(v);
+      for (int c = 0; c < V; ++c) ss = fmaf(v[j][c], v[j][c], ss);
+    }
+    ss = group_sum(ss, p.lanes);
+    if (!on) continue;
+    const float s = rsqrtf(fmaf(ss, p.inv_k, p.eps));
 #pragma unroll
-          for (int c = 0; c < V; ++c) {
-            out[c] = s * (e[u][j][c] * w[j][c] - v[c] * m);
-            dw[j][c] = fmaf(e[u][j][c] * v[c], s, dw[j][c]);
+    for (int j = 0; j < J; ++j) {
+      const int e0 = (l + j * p.lanes) * V;
+      if (e0 < p.K) {
+        float out[V], o[V];
+        mul_n<V>(out, v[j], w[j]);
+        if (rot[j].on) {
+          if (p.pairs && V > 1) {
+#pragma unroll
+            for (int c = 0; c < V; ++c) o[c] = v[j][c ^ (V > 1 ? 1 : 0)];
+          } else {
+            const int pc = rot[j].p0 / V;  // the partner's vector: lane pc % lanes, slot pc / lanes
+            ring.v[i % kSlots][0][J == 1 ? 0 : pc / p.lanes][base + (J == 1 ? pc : pc & (p.lanes - 1))].get(o);
           }
-          Vx<T, V>::store(dx + (h0 + i + u) * p.K + e0, out);
+          fma_n<V>(out, o, pw[j]);
         }
+        float s_n[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) s_n[c] = s;
+        mul_n<V>(out, out, s_n);
+        Vx<T, V>::store(out_at.at + e0, out);
       }
     }
+    out_at.next(p);
   }
 }
 
-// Each block keeps its rows' dw terms and writes one partial row per weight.
+// Both sums of a row (x^2 and e x) come from the same loads.  Each block keeps its rows' dw terms and writes one partial
+// row per weight.
 template <typename T, int V, int J>
-__global__ void __launch_bounds__(256) k_qk_bwd(const P p) {
-  constexpr int HB = J == 1 ? 2 : 1;
-  const int lane = threadIdx.x & 31, l = lane & (p.lanes - 1), warp = threadIdx.x >> 5;
+__global__ void __launch_bounds__(kThreads) k_qk_bwd(const P p) {
+  __shared__ Ring<T, V, J, 2> ring;
+  const int tid = threadIdx.x, lane = tid & 31, l = lane & (p.lanes - 1), base = tid - l, warp = tid >> 5;
   const int rpw = 32 / p.lanes;
-  const int64_t units = p.tokens * p.nhg, step = (int64_t)gridDim.x * 8 * rpw;
-  const int64_t first = ((int64_t)blockIdx.x * 8 + warp) * rpw;
+  const int64_t units = p.tokens * p.nhg, step = (int64_t)gridDim.x * kWarps * rpw;
+  const int64_t first = ((int64_t)blockIdx.x * kWarps + warp) * rpw;
   float dw[2][J][V];
 #pragma unroll
   for (int g = 0; g < 2; ++g)
@@ -300,30 +277,114 @@ __global__ void __launch_bounds__(256) k_qk_bwd(const P p) {
     const int64_t unit = u0 + lane / p.lanes;
     const bool live = unit < units;
     const int64_t tok = live ? unit / p.nhg : 0;
-    const int h0 = live ? (int)(unit - tok * p.nhg) * p.hg : 0, h1 = h0 + p.hg;
+    const int h0 = live ? (int)(unit - tok * p.nhg) * p.hg : 0;
     const int b = (int)(tok / p.T), t = (int)(tok - (int64_t)b * p.T);
+    const int turns = live ? min(p.hg, p.H + p.HK - h0) : 0;
+    Walk<T> in(p, p.q, p.qs, p.k, p.ks, b, t, h0), gin(p, p.dyq, p.dqs, p.dyk, p.dks, b, t, h0);
+    Out<T> out_at(p, p.dq, p.dk, tok, h0);
+    auto ask = [&](int i) {
+      if (i < turns) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int e0 = (l + j * p.lanes) * V;
+          if (e0 < p.K) {
+            Raw<T, V>&tx = ring.v[i % kSlots][0][j][tid], &tg = ring.v[i % kSlots][1][j][tid];
+            if constexpr (V == 1) {
+              tx.load(in.at + e0);
+              tg.load(gin.at + e0);
+            } else {
+              copy_async<Raw<T, V>::B>(&tx, in.at + e0);
+              copy_async<Raw<T, V>::B>(&tg, gin.at + e0);
+            }
+          }
+        }
+        in.next(p);
+        gin.next(p);
+      }
+      copies_commit();
+    };
+    __syncwarp();  // the unit before it has been read
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ask(i);
     const int64_t pos = position(p, b, t);
     Rot<V> rot[J];
+    float w[J][V];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int e0 = (l + j * p.lanes) * V;
       rot[j] = rotation<V>(p, e0 < p.K ? e0 : p.K, pos, -1.f);
     }
-    const int q1 = min(h1, p.H), k0 = max(h0, p.H) - p.H, k1 = min(h1, p.H + p.HK) - p.H;
-    const int qn = __reduce_max_sync(0xffffffffu, live ? max(q1 - h0, 0) : 0);
-    const int kn = __reduce_max_sync(0xffffffffu, live ? max(k1 - k0, 0) : 0);
-    if (qn > 0)
-      heads_bwd<T, V, J, HB>(p, static_cast<const T*>(p.q) + b * p.qs[0] + t * p.qs[1], p.qs[2],
-                             static_cast<const T*>(p.dyq) + b * p.dqs[0] + t * p.dqs[1], p.dqs[2],
-                             static_cast<T*>(p.dq) + tok * p.H * p.K, p.qw, h0, q1, qn, live, l, rot, dw[0]);
-    if (kn > 0)
-      heads_bwd<T, V, J, HB>(p, static_cast<const T*>(p.k) + b * p.ks[0] + t * p.ks[1], p.ks[2],
-                             static_cast<const T*>(p.dyk) + b * p.dks[0] + t * p.dks[1], p.dks[2],
-                             static_cast<T*>(p.dk) + tok * p.HK * p.K, p.kw, k0, k1, kn, live, l, rot, dw[1]);
+    int of = -1;
+    for (int i = 0; i < p.hg; ++i) {
+      copies_wait<kAhead - 1>();
+      __syncwarp();
+      ask(i + kAhead);
+      const bool on = i < turns, isq = out_at.h < p.H;
+      if (of != (int)isq) {
+        of = isq;
+#pragma unroll
+        for (int j = 0; j < J; ++j) weights<T, V>(isq ? p.qw : p.kw, p, (l + j * p.lanes) * V, w[j]);
+      }
+      float v[J][V], e[J][V], ss = 0.f, ex = 0.f;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[j][c] = e[j][c] = 0.f;
+        if (on && (l + j * p.lanes) * V < p.K) {
+          ring.v[i % kSlots][0][j][tid].get(v[j]);
+          ring.v[i % kSlots][1][j][tid].get(e[j]);
+          if (rot[j].on) {
+            float o[V];
+            if (p.pairs && V > 1) {
+#pragma unroll
+              for (int c = 0; c < V; ++c) o[c] = e[j][c ^ (V > 1 ? 1 : 0)];
+            } else {
+              const int pc = rot[j].p0 / V;
+              ring.v[i % kSlots][1][J == 1 ? 0 : pc / p.lanes][base + (J == 1 ? pc : pc & (p.lanes - 1))].get(o);
+            }
+            mul_n<V>(e[j], e[j], rot[j].c);
+            fma_n<V>(e[j], o, rot[j].s);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+          ss = fmaf(v[j][c], v[j][c], ss);
+          ex = fmaf(e[j][c] * w[j][c], v[j][c], ex);
+        }
+      }
+      ss = group_sum(ss, p.lanes);
+      ex = group_sum(ex, p.lanes);
+      if (!on) continue;
+      const float s = rsqrtf(fmaf(ss, p.inv_k, p.eps));
+      const float m = s * s * s * ex * p.inv_k;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int e0 = (l + j * p.lanes) * V;
+        if (e0 < p.K) {
+          float out[V];
+#pragma unroll
+          for (int c = 0; c < V; ++c) {
+            out[c] = fmaf(e[j][c] * w[j][c], s, -v[j][c] * m);
+            e[j][c] *= v[j][c] * s;
+          }
+          Vx<T, V>::store(out_at.at + e0, out);
+        }
+        if (isq) {
+#pragma unroll
+          for (int c = 0; c < V; ++c) dw[0][j][c] += e[j][c];
+        } else {
+#pragma unroll
+          for (int c = 0; c < V; ++c) dw[1][j][c] += e[j][c];
+        }
+      }
+      out_at.next(p);
+    }
   }
   if (p.part == nullptr) return;
   // rows of the block: fold the groups of a warp, then the warps, in a fixed order
-  __shared__ float red[8][2][256];
+  __syncthreads();
+  float(*red)[2][256] = reinterpret_cast<float(*)[2][256]>(&ring);  // [kWarps]
+  static_assert(sizeof(ring) >= kWarps * 2 * 256 * sizeof(float), "the ring holds the partial sums");
 #pragma unroll
   for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -336,10 +397,10 @@ __global__ void __launch_bounds__(256) k_qk_bwd(const P p) {
         if (lane < p.lanes && el < p.K) red[warp][g][el] = a;
       }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.K; i += 256) {
+  for (int i = threadIdx.x; i < 2 * p.K; i += kThreads) {
     const int g = i / p.K, el = i - g * p.K;
     float a = 0.f;
-    for (int w8 = 0; w8 < 8; ++w8) a += red[w8][g][el];
+    for (int w = 0; w < kWarps; ++w) a += red[w][g][el];
     p.part[(int64_t)blockIdx.x * 2 * p.K + i] = a;
   }
 }
@@ -378,7 +439,7 @@ P params(const tops_gla_qk_norm_args* a) {
   p.tokens = (int64_t)a->B * a->T;
   p.T = a->T; p.H = a->H; p.HK = a->HK; p.K = a->K; p.R = a->R;
   p.pairs = a->interleaved; p.wdtype = a->w_dtype; p.pos64 = a->positions_int64; p.table = a->table_rows;
-  p.eps = a->eps;
+  p.eps = a->eps; p.inv_k = 1.f / (float)a->K;
   p.q = a->q; p.k = a->k; p.qw = a->q_weight; p.kw = a->k_weight;
   for (int i = 0; i < 3; ++i) {
     p.qs[i] = a->q_strides[i];
@@ -387,6 +448,7 @@ P params(const tops_gla_qk_norm_args* a) {
   p.cos = a->cos_table; p.sin = a->sin_table;
   p.pos = a->positions; p.pb = a->positions_stride_b;
   p.yq = a->q_out; p.yk = a->k_out;
+  p.tvec = aligned_to(a->cos_table, 16) && aligned_to(a->sin_table, 16);
   p.wvec = aligned_to(a->q_weight, 16) && aligned_to(a->k_weight, 16);
   return p;
 }
@@ -435,7 +497,7 @@ int by_type(int dtype, int v, F f) {
 }
 
 constexpr int64_t kWant = 148 * 2048;
-constexpr int kBwdBlocks = 148 * 2;
+constexpr int kBwdBlocks = 148 * 4;
 
 }  // namespace qkn
 }  // namespace tops
@@ -452,12 +514,12 @@ TOPS_API int tops_gla_qk_norm_rotary_fwd(const tops_gla_qk_norm_args* a, void* s
   P p = params(a);
   const int v = vector_of(p, dtype_bytes(a->dtype), false);
   split(p, v, kWant);
-  const int64_t units = p.tokens * p.nhg, per_block = 8 * (32 / p.lanes);
+  const int64_t units = p.tokens * p.nhg, per_block = kWarps * (32 / p.lanes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchTimer lt(st, "qk_norm_fwd");
   by_type(a->dtype, v, [&](auto t, auto vv, auto jj) {
     k_qk_fwd<decltype(t), decltype(vv)::value, decltype(jj)::value>
-        <<<(unsigned)((units + per_block - 1) / per_block), 256, 0, st>>>(p);
+        <<<(unsigned)((units + per_block - 1) / per_block), kThreads, 0, st>>>(p);
     return 0;
   });
   TOPS_CUDA_LAUNCH_CHECK("qk_norm_fwd");
@@ -491,11 +553,11 @@ TOPS_API int tops_gla_qk_norm_rotary_bwd(const tops_gla_qk_norm_bwd_args* a, voi
   if (rows) {
     const int v = vector_of(p, dtype_bytes(f.dtype), true);
     split(p, v, kWant);
-    const int64_t units = p.tokens * p.nhg, per_block = 8 * (32 / p.lanes);
+    const int64_t units = p.tokens * p.nhg, per_block = kWarps * (32 / p.lanes);
     blocks = (int)std::min<int64_t>(kBwdBlocks, (units + per_block - 1) / per_block);
     LaunchTimer lt(st, "qk_norm_bwd");
     by_type(f.dtype, v, [&](auto t, auto vv, auto jj) {
-      k_qk_bwd<decltype(t), decltype(vv)::value, decltype(jj)::value><<<blocks, 256, 0, st>>>(p);
+      k_qk_bwd<decltype(t), decltype(vv)::value, decltype(jj)::value><<<blocks, kThreads, 0, st>>>(p);
       return 0;
     });
     TOPS_CUDA_LAUNCH_CHECK("qk_norm_bwd");

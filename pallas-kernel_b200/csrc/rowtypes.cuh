@@ -81,6 +81,22 @@ struct Raw {
   }
 };
 
+// copies of 8 or 16 bytes (or several of 16) from global to shared memory, in groups that are waited for by their order
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  const uint32_t a = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (BYTES > 16) {
+    copy_async<16>(dst, src);
+    copy_async<BYTES - 16>(static_cast<char*>(dst) + 16, static_cast<const char*>(src) + 16);
+  } else if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(a), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int AHEAD>
+__device__ __forceinline__ void copies_wait() {  // all but the last AHEAD groups have arrived
+  asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
+}
+
 // element i of a small parameter tensor stored in `dtype` (enum tops_dtype)
 __device__ __forceinline__ float load_param(const void* p, int dtype, int64_t i) {
   if (dtype == TOPS_F32) return static_cast<const float*>(p)[i];

@@ -230,27 +230,38 @@ __global__ void __launch_bounds__(kFwdThreads) k_scan_fwd(const P p) {
 }
 
 // One token of each of B rows: the state is read and written once (HBM bounds it).  Q lanes share a channel, four
-// states each (16 bytes of the state), and take R rows of the batch one after another, their states loaded together:
-// A, the bias and the skip weight are read once for them.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_scan_step(const P p, int Q, int R) {
+// states each (16 bytes of the state), and take four rows of the batch at a time, whose loads are in flight together; A
+// is read once for them.  What a row needs once per channel (delta, the gate, the output) is one lane's work: the lane
+// that the fold of the four rows' sums leaves that row with.
+template <typename T, int Q, bool VEC>
+__global__ void __launch_bounds__(256) k_scan_step(const P p, int R) {
+  constexpr int U = 4, OWN = Q >= U ? 1 : U / Q;  // rows at a time, and of them a lane's own
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, ch = id / Q;
-  const int nq = (int)(id - ch * Q), n0 = nq * 4;
+  const int lane = threadIdx.x & 31, nq = lane % Q, n0 = nq * 4;
   const bool on = ch < p.D;
   const int d = on ? (int)ch : 0, grp = d / (p.D / p.G), cnt = min(4, p.N - n0);
+  // own rows begin at `mine`, as fold() leaves them; the owner of row u is lane owner(u) of the channel
+  const int mine = Q == 1 ? 0 : Q == 2 ? nq * 2 : (nq & 1) * 2 + (nq >> 1 & 1);
+  auto owner = [](int u) { return Q == 1 ? 0 : Q == 2 ? u >> 1 : (u >> 1) + (u & 1) * 2; };
   float A[4];
+  if (VEC) {
+    const float4 v = on && cnt > 0 ? *reinterpret_cast<const float4*>(p.A + (int64_t)d * p.N + n0) : make_float4(0.f, 0.f, 0.f, 0.f);
+    A[0] = v.x; A[1] = v.y; A[2] = v.z; A[3] = v.w;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) A[i] = on && i < cnt ? p.A[(int64_t)d * p.N + n0 + i] * kLog2e : 0.f;
+    for (int i = 0; i < 4; ++i) A[i] = on && i < cnt ? p.A[(int64_t)d * p.N + n0 + i] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) A[i] *= kLog2e;
   const float bias = p.bias ? p.bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
-  const int b0 = blockIdx.y * R;
-  constexpr int U = 4;
-  for (int bb = b0; bb < min(b0 + R, p.B); bb += U) {
-    float h[U][4];
-    float x[U], dt[U], z[U], Bv[U][4], Cv[U][4];
+  const int b0 = blockIdx.y * R, b1 = min(b0 + R, p.B);
+  for (int bb = b0; bb < b1; bb += U) {
+    float h[U][4], x[OWN], z[OWN], dl[OWN];
+    Quad<T> bq[U], cq[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int b = bb + u;
-      const bool row = on && cnt > 0 && b < min(b0 + R, p.B);
+      const bool row = on && cnt > 0 && b < b1;
       const float* hp = p.h0 + ((int64_t)b * p.D + d) * p.N + n0;
       if (VEC) {
         const float4 v = row ? *reinterpret_cast<const float4*>(hp) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -259,46 +270,56 @@ __global__ void __launch_bounds__(256) k_scan_step(const P p, int Q, int R) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[u][i] = row && i < cnt ? hp[i] : 0.f;
       }
-      x[u] = row ? to_f<T>(static_cast<const T*>(p.x)[b * p.xs[0] + d]) : 0.f;
-      dt[u] = row ? to_f<T>(static_cast<const T*>(p.dt)[b * p.ds[0] + d]) : 0.f;
-      z[u] = row && p.z ? to_f<T>(static_cast<const T*>(p.z)[b * p.zs[0] + d]) : 0.f;
-      Quad<T> bq, cq;
-      quad_load<T>(static_cast<const T*>(p.bm) + b * p.bs[0] + grp * p.N + n0, p.vb, row ? cnt : 0, bq);
-      quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + grp * p.N + n0, p.vc, row ? cnt : 0, cq);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        Bv[u][i] = bq.get(i);
-        Cv[u][i] = cq.get(i);
-      }
+      quad_load<T>(static_cast<const T*>(p.bm) + b * p.bs[0] + grp * p.N + n0, p.vb, row ? cnt : 0, bq[u]);
+      quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + grp * p.N + n0, p.vc, row ? cnt : 0, cq[u]);
     }
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const int b = bb + mine + o;
+      const bool row = on && b < b1;
+      x[o] = row ? to_f<T>(static_cast<const T*>(p.x)[b * p.xs[0] + d]) : 0.f;
+      dl[o] = row ? to_f<T>(static_cast<const T*>(p.dt)[b * p.ds[0] + d]) : 0.f;
+      z[o] = row && p.z ? to_f<T>(static_cast<const T*>(p.z)[b * p.zs[0] + d]) : 0.f;
+    }
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      dl[o] += bias;
+      if (p.softplus) dl[o] = softplus(dl[o]);
+    }
+    float ys[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int b = bb + u;
-      const bool row = on && cnt > 0 && b < min(b0 + R, p.B);
-      float dl = dt[u] + bias;
-      if (p.softplus) dl = softplus(dl);
-      const float du = dl * x[u];
-      float y = 0.f;
+      float delta = dl[u % OWN], du = dl[u % OWN] * x[u % OWN];
+      if (Q > 1) {
+        delta = __shfl_sync(0xffffffffu, delta, owner(u), Q);
+        du = __shfl_sync(0xffffffffu, du, owner(u), Q);
+      }
+      ys[u] = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        h[u][i] = fmaf(ex2(fmaf(dl, A[i], kEx2Mean)), h[u][i], du * Bv[u][i]);
-        y = fmaf(Cv[u][i], h[u][i], y);
+        h[u][i] = fmaf(ex2(fmaf(delta, A[i], kEx2Mean)), h[u][i], du * bq[u].get(i));
+        ys[u] = fmaf(cq[u].get(i), h[u][i], ys[u]);
       }
-      for (int o = 1; o < Q; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-      if (!row) continue;
-      float* ho = p.ht + ((int64_t)b * p.D + d) * p.N + n0;
-      if (VEC) {
-        *reinterpret_cast<float4*>(ho) = make_float4(h[u][0], h[u][1], h[u][2], h[u][3]);
-      } else {
+      if (on && cnt > 0 && b < b1) {
+        float* ho = p.ht + ((int64_t)b * p.D + d) * p.N + n0;
+        if (VEC) {
+          *reinterpret_cast<float4*>(ho) = make_float4(h[u][0], h[u][1], h[u][2], h[u][3]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < cnt) ho[i] = h[u][i];
+          for (int i = 0; i < 4; ++i)
+            if (i < cnt) ho[i] = h[u][i];
+        }
       }
-      if (nq == 0) {
-        y = fmaf(skip, x[u], y);
-        if (p.z) y *= z[u] * fast_sigmoid(z[u]);
-        static_cast<T*>(p.y)[(int64_t)b * p.D + d] = from_f<T>(y);
-      }
+    }
+    fold<U, Q, 1>(ys, lane);
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const int b = bb + mine + o;
+      if (!on || b >= b1 || nq >= U) continue;
+      float y = fmaf(skip, x[o], ys[o]);
+      if (p.z) y *= z[o] * fast_sigmoid(z[o]);
+      static_cast<T*>(p.y)[(int64_t)b * p.D + d] = from_f<T>(y);
     }
   }
 }
@@ -371,20 +392,25 @@ TOPS_API int tops_gla_ssm_scan_step(const tops_gla_scan_args* a, void* stream) {
   const P p = params(a);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchTimer lt(st, "ssm_scan_step");
-  int Q = 1;  // lanes of a channel: a power of two, so that a channel lies in one warp
-  while (Q * 4 < p.N) Q *= 2;
-  const int blocks = (int)(((int64_t)p.D * Q + 255) / 256);
-  // rows of a thread: all loads of four are in flight at once; fewer where the grid would not fill the SMs
-  int R = 4;
-  while (R > 1 && (int64_t)blocks * ((p.B + R - 1) / R) < 148 * 4) R /= 2;
-  R = std::max(R, (p.B + 65534) / 65535);
-  const bool vec = p.N % 4 == 0 && aligned_to(p.h0, 16) && aligned_to(p.ht, 16);
+  // lanes of a channel: a power of two, so that a channel lies in one warp.  Every call pays a launch's latency; more rows
+  // a thread than four at once only pay where the grid fills the SMs several times over.
+  const bool vec = p.N % 4 == 0 && aligned_to(p.h0, 16) && aligned_to(p.ht, 16) && aligned_to(p.A, 16);
   by_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid(blocks, (p.B + R - 1) / R);
-    if (vec) k_scan_step<T, true><<<grid, 256, 0, st>>>(p, Q, R);
-    else k_scan_step<T, false><<<grid, 256, 0, st>>>(p, Q, R);
-    return 0;
+    auto go = [&](auto lanes) {
+      constexpr int Q = decltype(lanes)::value;
+      const int blocks = (int)(((int64_t)p.D * Q + 255) / 256);
+      const int R = std::max(4, ((p.B + 65534) / 65535 + 3) / 4 * 4);
+      const dim3 grid(blocks, (p.B + R - 1) / R);
+      if (vec) k_scan_step<T, Q, true><<<grid, 256, 0, st>>>(p, R);
+      else k_scan_step<T, Q, false><<<grid, 256, 0, st>>>(p, R);
+      return 0;
+    };
+    if (p.N <= 4) return go(std::integral_constant<int, 1>());
+    if (p.N <= 8) return go(std::integral_constant<int, 2>());
+    if (p.N <= 16) return go(std::integral_constant<int, 4>());
+    if (p.N <= 32) return go(std::integral_constant<int, 8>());
+    return go(std::integral_constant<int, 16>());
   });
   TOPS_CUDA_LAUNCH_CHECK("ssm_scan_step");
   return TOPS_OK;
