@@ -251,7 +251,8 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the handle without the Stream object around it: 0.2 instead of 2.3 us a call
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def launch_count() -> int:

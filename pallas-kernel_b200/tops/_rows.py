@@ -2,13 +2,9 @@
 (``causal_conv1d``, ``selective_scan``, ``qk_norm_rotary`` and their single-token forms)."""
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _C
-
-_NOTHING = contextlib.nullcontext()
 
 
 def check_cuda(op: str, first: torch.Tensor, **others) -> None:
@@ -31,24 +27,33 @@ def check_like(op: str, name: str, t: torch.Tensor | None, shape: tuple, dtype: 
 
 
 def no_grad_only(op: str, other: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if wants_grad(*tensors):
         raise RuntimeError(f"{op} has no gradient: call {other}, or this under torch.no_grad()")
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def rows(t: torch.Tensor | None, inner: int = 1) -> torch.Tensor | None:
-    """``t`` itself where its last ``inner`` dims are dense, else a contiguous copy."""
-    if t is None or t.is_contiguous():
+def like(t: torch.Tensor | None, shape, dtype: torch.dtype, device: int) -> bool:
+    """Whether ``t`` is absent or has that shape, dtype and device (the quick form of the checks below)."""
+    return t is None or (t.shape == shape and t.dtype == dtype and t.get_device() == device)
+
+
+def rows(t: torch.Tensor | None) -> torch.Tensor | None:
+    """``t`` itself where its last dim is dense, else a contiguous copy."""
+    return t if t is None or t.stride(-1) == 1 or t.is_contiguous() else t.contiguous()
+
+
+def rows2(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself where its last two dims are dense, else a contiguous copy."""
+    if t.stride(-1) == 1 and (t.shape[-2] == 1 or t.stride(-2) == t.shape[-1]):
         return t
-    want = 1
-    for i in range(1, inner + 1):
-        if t.shape[-i] != 1 and t.stride(-i) != want:
-            return t.contiguous()
-        want *= t.shape[-i]
-    return t
+    return t.contiguous()
 
 
 def sequences(op: str, cu_seqlens, B: int, T: int, device) -> tuple[int, torch.Tensor | None]:
@@ -94,9 +99,13 @@ def state_target(op: str, state: torch.Tensor, out: torch.Tensor | None, *reads)
     return (state if same else state.contiguous()), out
 
 
-def on_device(t: torch.Tensor):
-    """The launches of a call go to its tensors' device, whatever the current one is."""
-    return _NOTHING if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def launch(name: str, args, t: torch.Tensor) -> None:
+    """One C call on the current stream of ``t``'s device, whatever the current device is."""
+    if t.get_device() == torch.cuda.current_device():
+        _C.call(name, args, _C.stream_of(t))
+    else:
+        with torch.cuda.device(t.device):
+            _C.call(name, args, _C.stream_of(t))
 
 
 def workspace(nbytes: int, t: torch.Tensor) -> torch.Tensor | None:

@@ -31,8 +31,7 @@ def _forward(x, w, bias, state, act, want_final, N, cu):
     w, bias, state = (t if t is None else t.contiguous() for t in (w, bias, state))
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     final = torch.empty(N, x.shape[2], w.shape[1] - 1, dtype=x.dtype, device=x.device) if want_final else None
-    with _rows.on_device(x):
-        _C.call("tops_gla_causal_conv_fwd", _args(x, w, bias, state, y, final, act, N, cu), _C.stream_of(x))
+    _rows.launch("tops_gla_causal_conv_fwd", _args(x, w, bias, state, y, final, act, N, cu), x)
     return y, final
 
 
@@ -82,16 +81,19 @@ class _CausalConv(torch.autograd.Function):
                            dy.stride(1), _C.ptr(dfinal), dx.data_ptr(), _C.ptr(dw), _C.ptr(db), _C.ptr(ds), None, 0)
         ws = _rows.workspace(_C.lib().tops_gla_causal_conv_bwd_workspace_size(a), x)
         a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
-        with _rows.on_device(x):
-            _C.call("tops_gla_causal_conv_bwd", a, _C.stream_of(x))
+        _rows.launch("tops_gla_causal_conv_bwd", a, x)
         return dx, dw, db, ds, None, None, None, None
 
 
 def _check(op, x, weight, bias, activation, D, state, state_shape):
     if activation not in _ACT:
         raise ValueError(f"{op}: activation must be None, 'silu' or 'swish', got {activation!r}")
+    W, dev, wd = weight.shape[1], x.get_device(), weight.dtype
+    if (dev >= 0 and x.dtype in _C._DTYPE and W in KERNEL_WIDTHS and weight.shape[0] == D and weight.get_device() == dev
+            and (wd == x.dtype or wd == torch.float32) and (bias is None or _rows.like(bias, (D,), wd, dev))
+            and (state is None or _rows.like(state, (*state_shape, D, W - 1), x.dtype, dev))):
+        return
     _rows.check_cuda(op, x, weight=weight, bias=bias, state=state)
-    W = weight.shape[1]
     if W not in KERNEL_WIDTHS:
         raise ValueError(f"{op}: the kernel width must be one of {KERNEL_WIDTHS}, got {W}")
     if weight.dtype not in (x.dtype, torch.float32):
@@ -156,8 +158,7 @@ def causal_conv1d_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     a = _C.ConvArgs(B, 1, D, weight.shape[1], B, _C.dtype_code(x.dtype), _C.dtype_code(weight.dtype), _ACT[activation],
                     None, x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _C.ptr(bias), state.data_ptr(), y.data_ptr(),
                     out.data_ptr())
-    with _rows.on_device(x):
-        _C.call("tops_gla_causal_conv_step", a, _C.stream_of(x))
+    _rows.launch("tops_gla_causal_conv_step", a, x)
     return y, out
 
 

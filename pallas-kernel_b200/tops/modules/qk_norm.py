@@ -26,8 +26,11 @@ def rotary_tables(max_positions: int, rotary_dim: int, base: float = 10000.0, de
     return angle.cos().float(), angle.sin().float()
 
 
+_S3 = _C.C.c_int64 * 3
+
+
 def _strides(t):
-    return (_C.C.c_int64 * 3)(*t.stride()[:3])
+    return _S3(*t.stride()[:3])
 
 
 def _args(q, k, qw, kw, cos, sin, positions, eps, interleaved):
@@ -48,8 +51,7 @@ def _forward(q, k, qw, kw, cos, sin, positions, eps, interleaved):
     ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
     a = _args(q, k, qw, kw, cos, sin, positions, eps, interleaved)
     a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
-    with _rows.on_device(q):
-        _C.call("tops_gla_qk_norm_rotary_fwd", a, _C.stream_of(q))
+    _rows.launch("tops_gla_qk_norm_rotary_fwd", a, q)
     return qo, ko
 
 
@@ -76,9 +78,47 @@ class _QKNormRotary(torch.autograd.Function):
                              dk.data_ptr(), _C.ptr(dqw), _C.ptr(dkw), None, 0)
         ws = _rows.workspace(_C.lib().tops_gla_qk_norm_rotary_bwd_workspace_size(a), q)
         a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
-        with _rows.on_device(q):
-            _C.call("tops_gla_qk_norm_rotary_bwd", a, _C.stream_of(q))
+        _rows.launch("tops_gla_qk_norm_rotary_bwd", a, q)
         return dq, dk, dqw, dkw, None, None, None, None, None
+
+
+def _check(op, q, k, q_weight, k_weight, cos, sin, positions):
+    """-> the weights in one dtype, the tables and positions as the kernel takes them."""
+    B, T, _, K = q.shape
+    dev, dt = q.get_device(), q.dtype
+    wd = dt if q_weight is None else q_weight.dtype
+    if not (dev >= 0 and dt in _C._DTYPE and _rows.like(k, (B, T, k.shape[2], K), dt, dev) and (wd == dt or wd == torch.float32)
+            and _rows.like(q_weight, (K,), wd, dev) and _rows.like(k_weight, (K,), wd, dev)):
+        _rows.check_cuda(op, q, k=k, q_weight=q_weight, k_weight=k_weight)
+        _rows.check_like(op, "k", k, (B, T, k.shape[2], K), dt)
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None:
+                assert tuple(w.shape) == (K,), f"{op}: expected {name} shape {(K,)}, got {tuple(w.shape)}"
+                if w.dtype not in (dt, torch.float32):
+                    raise TypeError(f"{op}: {name} must be {dt} or float32, got {w.dtype}")
+        if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+            q_weight, k_weight = q_weight.float(), k_weight.float()
+    assert (cos is None) == (sin is None), f"{op}: cos and sin come together"
+    if cos is None:
+        return q_weight, k_weight, None, None, None
+    _rows.check_cuda(op, q, cos=cos, sin=sin, positions=positions)
+    R = 2 * cos.shape[-1]
+    assert cos.dim() == 2 and cos.shape[0] > 0 and 0 < R <= K, \
+        f"{op}: expected cos [P, R / 2] with R in 2..{K}, got {tuple(cos.shape)}"
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.shape != cos.shape or t.dtype != torch.float32:
+            _rows.check_like(op, name, t, cos.shape, torch.float32)
+        if t.requires_grad:
+            raise RuntimeError(f"{op}: {name} has no gradient")
+    if positions is None:
+        assert T <= cos.shape[0], f"{op}: {T} rows, but the tables have {cos.shape[0]}"
+    else:
+        assert positions.shape == (B, T) or positions.shape == (T,), \
+            f"{op}: expected positions [T] or [B, T], got {tuple(positions.shape)}"
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{op}: positions must be int32 or int64, got {positions.dtype}")
+        positions = _rows.rows(positions)
+    return q_weight, k_weight, cos.contiguous(), sin.contiguous(), positions
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None = None,
@@ -103,34 +143,6 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     B, T, _, K = q.shape
     if not 1 <= K <= MAX_HEAD:
         raise ValueError(f"{op}: heads must have 1 to {MAX_HEAD} elements, got {K}")
-    _rows.check_cuda(op, q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions)
-    _rows.check_like(op, "k", k, (B, T, k.shape[2], K), q.dtype)
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            assert tuple(w.shape) == (K,), f"{op}: expected {name} shape {(K,)}, got {tuple(w.shape)}"
-            if w.dtype not in (q.dtype, torch.float32):
-                raise TypeError(f"{op}: {name} must be {q.dtype} or float32, got {w.dtype}")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        q_weight, k_weight = q_weight.float(), k_weight.float()
-    assert (cos is None) == (sin is None), f"{op}: cos and sin come together"
-    if cos is not None:
-        R = 2 * cos.shape[-1]
-        assert cos.dim() == 2 and cos.shape[0] > 0 and 0 < R <= K, \
-            f"{op}: expected cos [P, R / 2] with R in 2..{K}, got {tuple(cos.shape)}"
-        for name, t in (("cos", cos), ("sin", sin)):
-            _rows.check_like(op, name, t, cos.shape, torch.float32)
-            if t.requires_grad:
-                raise RuntimeError(f"{op}: {name} has no gradient")
-        cos, sin = cos.contiguous(), sin.contiguous()
-        if positions is None:
-            assert T <= cos.shape[0], f"{op}: {T} rows, but the tables have {cos.shape[0]}"
-        else:
-            assert tuple(positions.shape) in ((T,), (B, T)), \
-                f"{op}: expected positions [T] or [B, T], got {tuple(positions.shape)}"
-            if positions.dtype not in (torch.int32, torch.int64):
-                raise TypeError(f"{op}: positions must be int32 or int64, got {positions.dtype}")
-            positions = _rows.rows(positions)
-    else:
-        positions = None
+    q_weight, k_weight, cos, sin, positions = _check(op, q, k, q_weight, k_weight, cos, sin, positions)
     a = (q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved))
     return _QKNormRotary.apply(*a) if _rows.wants_grad(q, k, q_weight, k_weight) else _forward(*a)

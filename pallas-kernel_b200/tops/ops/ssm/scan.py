@@ -20,8 +20,19 @@ __all__ = ["selective_scan", "selective_scan_step"]
 MAX_STATES = 64
 
 
+_S2 = _C.C.c_int64 * 2
+
+
 def _strides(t):
-    return (_C.C.c_int64 * 2)(0, 0) if t is None else (_C.C.c_int64 * 2)(t.stride(0), t.stride(1))
+    return _S2() if t is None else _S2(t.stride(0), t.stride(1))
+
+
+def _row_stride(t):
+    return _S2() if t is None else _S2(t.stride(0))
+
+
+def _f32(t):
+    return t if t is None or t.dtype == torch.float32 else t.float()
 
 
 def _args(x, dt, A, Bm, Cm, D, z, bias, h0, softplus, S, cu):
@@ -33,9 +44,9 @@ def _args(x, dt, A, Bm, Cm, D, z, bias, h0, softplus, S, cu):
 
 
 def _dense(x, dt, A, Bm, Cm, D, z, bias, h0):
-    r = _rows.rows
+    r, r2 = _rows.rows, _rows.rows2
     c = [None if t is None else t.contiguous() for t in (A, D, bias, h0)]
-    return r(x), r(dt), c[0], r(Bm, 2), r(Cm, 2), c[1], r(z), c[2], c[3]
+    return r(x), r(dt), c[0], r2(Bm), r2(Cm), c[1], r(z), c[2], c[3]
 
 
 def _forward(x, dt, A, Bm, Cm, D, z, bias, h0, softplus, want_final, S, cu, save):
@@ -48,10 +59,9 @@ def _forward(x, dt, A, Bm, Cm, D, z, bias, h0, softplus, want_final, S, cu, save
     if save:
         states = torch.empty(L.tops_gla_ssm_scan_states_size(a) // 4, dtype=torch.float32, device=x.device)
     a.y, a.ht, a.states = y.data_ptr(), _C.ptr(ht), _C.ptr(states)
-    with _rows.on_device(x):
-        ws = _rows.workspace(L.tops_gla_ssm_scan_fwd_workspace_size(a), x)
-        a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
-        _C.call("tops_gla_ssm_scan_fwd", a, _C.stream_of(x))
+    ws = _rows.workspace(L.tops_gla_ssm_scan_fwd_workspace_size(a), x)
+    a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
+    _rows.launch("tops_gla_ssm_scan_fwd", a, x)
     return y, ht, states
 
 
@@ -85,33 +95,41 @@ class _SelectiveScan(torch.autograd.Function):
         f.states = states.data_ptr()
         a = _C.ScanBwdArgs(f, dout.data_ptr(), _strides(dout), _C.ptr(dht), dx.data_ptr(), ddt.data_ptr(), _C.ptr(dz),
                            dB.data_ptr(), dC.data_ptr(), _C.ptr(dA), _C.ptr(dD), _C.ptr(dbias), _C.ptr(dh0), None, 0)
-        with _rows.on_device(x):
-            ws = _rows.workspace(_C.lib().tops_gla_ssm_scan_bwd_workspace_size(a), x)
-            a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
-            _C.call("tops_gla_ssm_scan_bwd", a, _C.stream_of(x))
+        ws = _rows.workspace(_C.lib().tops_gla_ssm_scan_bwd_workspace_size(a), x)
+        a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
+        _rows.launch("tops_gla_ssm_scan_bwd", a, x)
         return dx, ddt, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None
 
 
 def _check(op, lead, x, dt, A, Bm, Cm, D, z, dt_bias, state, S):
     """-> (Bm, Cm) as [*lead, G, N], with every shape and type checked (``lead`` = x's leading dims)."""
-    ch = x.shape[-1]
+    shape, ch, n = x.shape, x.shape[-1], len(lead)
+    if Bm.dim() == n + 1:
+        Bm = Bm.unsqueeze(n)
+    if Cm.dim() == n + 1:
+        Cm = Cm.unsqueeze(n)
+    if Bm.dim() == n + 2 and A.dim() == 2:  # quick: all in one expression, explained below where it fails
+        N, G, dev, dtype = A.shape[1], Bm.shape[n], x.get_device(), x.dtype
+        like, bc = _rows.like, (*lead, Bm.shape[n], A.shape[1])
+        if (dev >= 0 and dtype in _C._DTYPE and 1 <= N <= MAX_STATES and G >= 1 and ch % G == 0 and like(dt, shape, dtype, dev)
+                and like(z, shape, dtype, dev) and like(Bm, bc, dtype, dev) and like(Cm, bc, dtype, dev)
+                and A.shape[0] == ch and A.get_device() == dev
+                and (D is None or (D.shape == (ch,) and D.get_device() == dev))
+                and (dt_bias is None or (dt_bias.shape == (ch,) and dt_bias.get_device() == dev))
+                and (state is None or (state.shape == (S, ch, N) and state.get_device() == dev))):
+            return Bm, Cm
     _rows.check_cuda(op, x, dt=dt, A=A, B=Bm, C=Cm, D=D, z=z, dt_bias=dt_bias, state=state)
     assert A.dim() == 2 and A.shape[0] == ch, f"{op}: expected A shape ({ch}, N), got {tuple(A.shape)}"
     N = A.shape[1]
     if not 1 <= N <= MAX_STATES:
         raise ValueError(f"{op}: a channel must have 1 to {MAX_STATES} states, got {N}")
-    n = len(lead)
-    if Bm.dim() == n + 1:
-        Bm = Bm.unsqueeze(n)
-    if Cm.dim() == n + 1:
-        Cm = Cm.unsqueeze(n)
     assert Bm.dim() == n + 2, f"{op}: expected B {tuple(lead) + (N,)} or with groups before N, got {tuple(Bm.shape)}"
     G = Bm.shape[n]
     assert G >= 1 and ch % G == 0, f"{op}: {ch} channels cannot be shared by {G} groups"
-    for name, t, shape in (("dt", dt, x.shape), ("z", z, x.shape), ("B", Bm, (*lead, G, N)), ("C", Cm, (*lead, G, N))):
-        _rows.check_like(op, name, t, shape, x.dtype)
-    for name, t, shape in (("A", A, (ch, N)), ("D", D, (ch,)), ("dt_bias", dt_bias, (ch,)), ("state", state, (S, ch, N))):
-        assert t is None or tuple(t.shape) == shape, f"{op}: expected {name} shape {shape}, got {tuple(t.shape)}"
+    for name, t, want in (("dt", dt, shape), ("z", z, shape), ("B", Bm, (*lead, G, N)), ("C", Cm, (*lead, G, N))):
+        _rows.check_like(op, name, t, want, x.dtype)
+    for name, t, want in (("A", A, (ch, N)), ("D", D, (ch,)), ("dt_bias", dt_bias, (ch,)), ("state", state, (S, ch, N))):
+        assert t is None or tuple(t.shape) == want, f"{op}: expected {name} shape {want}, got {tuple(t.shape)}"
     return Bm, Cm
 
 
@@ -135,7 +153,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     assert x.dim() == 3, f"{op}: expected x [B, T, D], got {tuple(x.shape)}"
     S, cu = _rows.sequences(op, cu_seqlens, x.shape[0], x.shape[1], x.device)
     B, C = _check(op, x.shape[:2], x, dt, A, B, C, D, z, dt_bias, initial_state, S)
-    A, D, dt_bias, h0 = (None if t is None else t.float() for t in (A, D, dt_bias, initial_state))
+    A, D, dt_bias, h0 = _f32(A), _f32(D), _f32(dt_bias), _f32(initial_state)
     tensors = (x, dt, A, B, C, D, z, dt_bias, h0)
     if not _rows.wants_grad(*tensors):
         y, ht, _ = _forward(*tensors, int(dt_softplus), bool(output_final_state), S, cu, False)
@@ -161,16 +179,16 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     if state.dtype != torch.float32:
         raise TypeError(f"{op}: state must be float32, got {state.dtype}")
     _rows.no_grad_only(op, "selective_scan", x, dt, A, B, C, state, D, z, dt_bias)
-    r = _rows.rows
-    x, dt, z, B, C = r(x), r(dt), r(z), r(B, 2), r(C, 2)
-    A, D, dt_bias = (None if t is None else t.float().contiguous() for t in (A, D, dt_bias))
+    r, r2 = _rows.rows, _rows.rows2
+    x, dt, z, B, C = r(x), r(dt), r(z), r2(B), r2(C)
+    A = _f32(A).contiguous()
+    D, dt_bias = (None if t is None else _f32(t).contiguous() for t in (D, dt_bias))
     state, out = _rows.state_target(op, state, state_out, x, dt, A, B, C, D, z, dt_bias)
     y = torch.empty(Bsz, ch, dtype=x.dtype, device=x.device)
     G, N = B.shape[1:]
-    s = lambda t: (_C.C.c_int64 * 2)(0 if t is None else t.stride(0), 0)  # noqa: E731
+    s = _row_stride
     a = _C.ScanArgs(Bsz, 1, ch, N, G, Bsz, _C.dtype_code(x.dtype), int(dt_softplus), None, x.data_ptr(), dt.data_ptr(),
                     _C.ptr(z), B.data_ptr(), C.data_ptr(), s(x), s(dt), s(z), s(B), s(C), A.data_ptr(), _C.ptr(D),
                     _C.ptr(dt_bias), state.data_ptr(), y.data_ptr(), out.data_ptr(), None, None, 0)
-    with _rows.on_device(x):
-        _C.call("tops_gla_ssm_scan_step", a, _C.stream_of(x))
+    _rows.launch("tops_gla_ssm_scan_step", a, x)
     return y, out
