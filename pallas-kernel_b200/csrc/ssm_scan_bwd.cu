@@ -479,28 +479,35 @@ __global__ void __launch_bounds__(128) k_scan_bwd_sum(const P p) {
   if (VAR && blockIdx.x == 0 && tid == 0) p.broken[k] = broken != 0;
 }
 
-// dB, dC [B, T, G, N] = the parts' sums, in a fixed order
+// The partial sums, each in a fixed order, in one launch: dB, dC [B, T, G, N] over the parts of a group (the first
+// `bc_blocks` blocks), dA, dD and dbias over batch rows and segments (the rest).
 template <typename T>
-__global__ void k_scan_bc(const P p, T* __restrict__ dB, T* __restrict__ dC) {
-  const int64_t rows = (int64_t)p.B * p.T, per = rows * 2 * p.N;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int grp = blockIdx.y;
-  if (i >= per) return;
+__global__ void __launch_bounds__(256) k_scan_fold(const P p, int64_t bc_blocks, T* __restrict__ dB, T* __restrict__ dC,
+                                                   float* __restrict__ dA, float* __restrict__ dskip,
+                                                   float* __restrict__ dbias) {
+  if (blockIdx.x < bc_blocks) {
+    const int64_t per = (int64_t)p.B * p.T * 2 * p.N, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= per * p.G) return;
+    const int grp = (int)(i / per);
+    const int64_t at = i - grp * per, row = at / (2 * p.N);
+    const int c = (int)(at - row * 2 * p.N);
+    const float* src = p.pbc + (int64_t)grp * p.parts * per + at;
+    float s = 0.f;
+    for (int k = 0; k < p.parts; ++k) s += src[k * per];
+    T* o = c < p.N ? dB : dC;
+    o[(row * p.G + grp) * p.N + (c < p.N ? c : c - p.N)] = from_f<T>(s);
+    return;
+  }
+  const int64_t dn = (int64_t)p.D * p.N, i = (blockIdx.x - bc_blocks) * 256 + threadIdx.x;
+  if (i >= dn + 2 * p.D) return;
+  const int64_t j = i - dn;  // dD, then dbias
+  float* o = i < dn ? dA + i : j < p.D ? dskip + j : dbias + (j - p.D);
+  if ((i < dn ? dA : j < p.D ? dskip : dbias) == nullptr) return;
+  const float* src = i < dn ? p.pa + i : p.pd + j;
+  const int64_t stride = i < dn ? dn : 2 * (int64_t)p.D;
   float s = 0.f;
-  for (int k = 0; k < p.parts; ++k) s += p.pbc[((int64_t)grp * p.parts + k) * per + i];
-  const int64_t row = i / (2 * p.N);
-  const int c = (int)(i - row * 2 * p.N);
-  T* o = c < p.N ? dB : dC;
-  o[(row * p.G + grp) * p.N + (c < p.N ? c : c - p.N)] = from_f<T>(s);
-}
-
-// out[i] = sum over parts of part[k][i], in a fixed order
-__global__ void k_scan_sum(int parts, int64_t n, int64_t stride, const float* __restrict__ part, float* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  float s = 0.f;
-  for (int k = 0; k < parts; ++k) s += part[k * stride + i];
-  out[i] = s;
+  for (int k = 0; k < p.B * p.nseg; ++k) s += src[k * stride];
+  *o = s;
 }
 
 size_t plan_bwd(P& p, void* ws) {
@@ -535,6 +542,7 @@ TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream
   TOPS_CHECK_ARG(!rows || (f.x && f.dt && f.Bm && f.Cm && f.A && f.states && a->dout && a->dx && a->ddt && a->dB && a->dC),
                  "ssm_scan_bwd: x, dt, B, C, A, states, dout and the gradients of x, dt, B and C are required");
   TOPS_CHECK_ARG(!rows || !f.z || a->dz, "ssm_scan_bwd: z needs dz");
+  TOPS_CHECK_ARG(aligned_to(a->workspace, 16), "ssm_scan_bwd: workspace must be 16-byte aligned");
   P p = params(&f);
   const size_t need = plan_bwd(p, a->workspace);
   if (need && (a->workspace == nullptr || a->workspace_bytes < need))
@@ -575,25 +583,16 @@ TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream
     if (rc) return rc;
     TOPS_CUDA_LAUNCH_CHECK("ssm_scan_bwd");
   }
-  if (rows) {
-    LaunchTimer lt(st, "ssm_scan_bc");
-    const int64_t per = (int64_t)p.B * p.T * 2 * p.N;
-    by_type(f.dtype, [&](auto t) {
-      using T = decltype(t);
-      k_scan_bc<T><<<dim3((unsigned)((per + 255) / 256), p.G), 256, 0, st>>>(p, static_cast<T*>(a->dB), static_cast<T*>(a->dC));
-      return 0;
-    });
-    TOPS_CUDA_LAUNCH_CHECK("ssm_scan_bc");
-  }
-  const struct { int64_t n, stride; const float* part; float* out; } sums[] = {
-      {(int64_t)p.D * p.N, (int64_t)p.D * p.N, p.pa, a->dA}, {p.D, 2 * (int64_t)p.D, p.pd, a->dskip},
-      {p.D, 2 * (int64_t)p.D, p.pd + p.D, a->ddt_bias}};
-  for (const auto& s : sums) {
-    if (!s.out) continue;
-    LaunchTimer lt(st, "ssm_scan_param");
-    k_scan_sum<<<(unsigned)((s.n + 255) / 256), 256, 0, st>>>(p.B * p.nseg, s.n, s.stride, s.part, s.out);
-    TOPS_CUDA_LAUNCH_CHECK("ssm_scan_param");
-  }
+  LaunchTimer lt(st, "ssm_scan_fold");
+  const int64_t bc = (int64_t)p.B * p.T * 2 * p.N * p.G, params_n = (int64_t)p.D * p.N + 2 * p.D;
+  const int64_t bc_blocks = (bc + 255) / 256;
+  by_type(f.dtype, [&](auto t) {
+    using T = decltype(t);
+    k_scan_fold<T><<<(unsigned)(bc_blocks + (params_n + 255) / 256), 256, 0, st>>>(
+        p, bc_blocks, static_cast<T*>(a->dB), static_cast<T*>(a->dC), a->dA, a->dskip, a->ddt_bias);
+    return 0;
+  });
+  TOPS_CUDA_LAUNCH_CHECK("ssm_scan_fold");
   return TOPS_OK;
 }
 

@@ -126,7 +126,9 @@ def test_scan_refusals_without_a_device(C):
                          ({"D": 0}, -1, "dimension"), ({"T": -1}, -1, "dimension"), ({"A": None}, -1, "required"),
                          ({"B": 70000, "S": 70000}, -2, "65535"),
                          ({"cu_seqlens": 16, "B": 2, "S": 2}, -1, "B == 1"),
-                         ({"cu_seqlens": 16, "S": 0}, -1, "sequences")):
+                         ({"cu_seqlens": 16, "S": 0}, -1, "sequences"), ({"ht": 24}, -1, "16-byte"),
+                         ({"states": 4}, -1, "16-byte"), ({"workspace": 8}, -1, "16-byte"),
+                         ({"D": 70000, "G": 70000}, -2, "65535 groups")):
         _refused(C, "tops_gla_ssm_scan_fwd", _scan(C, **kw), st, text)
     _refused(C, "tops_gla_ssm_scan_step", _scan(C), -1, "T must be 1")
     _refused(C, "tops_gla_ssm_scan_step", _scan(C, T=1), -1, "required")
