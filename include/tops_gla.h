@@ -473,7 +473,8 @@ typedef struct tops_gla_scan_args {
   int32_t B, T, D, N, G, S, dtype, softplus;
   const int32_t* cu_seqlens;
   const void* x; const void* dt; const void* z; const void* Bm; const void* Cm;
-  int64_t x_strides[2], dt_strides[2], z_strides[2], b_strides[2], c_strides[2];
+  int64_t x_stride_b, x_stride_t, dt_stride_b, dt_stride_t, z_stride_b, z_stride_t;
+  int64_t b_stride_b, b_stride_t, c_stride_b, c_stride_t;
   const float* A; const float* skip; const float* dt_bias; const float* h0;
   void* y; float* ht; float* states;
   void* workspace; size_t workspace_bytes;
@@ -484,7 +485,7 @@ typedef struct tops_gla_scan_args {
  * forward; f.y, f.ht and f.workspace are not used. */
 typedef struct tops_gla_scan_bwd_args {
   tops_gla_scan_args f;
-  const void* dout; int64_t dout_strides[2];
+  const void* dout; int64_t dout_stride_b, dout_stride_t;
   const float* dht;
   void* dx; void* ddt; void* dz; void* dB; void* dC;
   float* dA; float* dskip; float* ddt_bias; float* dh0;

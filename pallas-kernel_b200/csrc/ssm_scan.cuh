@@ -272,13 +272,11 @@ inline P params(const tops_gla_scan_args* a) {
   p.B = a->B; p.T = a->T; p.D = a->D; p.N = a->N; p.G = a->G; p.S = a->S; p.softplus = a->softplus;
   p.cu = a->cu_seqlens;
   p.x = a->x; p.dt = a->dt; p.z = a->z; p.bm = a->Bm; p.cm = a->Cm;
-  for (int i = 0; i < 2; ++i) {
-    p.xs[i] = a->x_strides[i];
-    p.ds[i] = a->dt_strides[i];
-    p.zs[i] = a->z_strides[i];
-    p.bs[i] = a->b_strides[i];
-    p.cs[i] = a->c_strides[i];
-  }
+  p.xs[0] = a->x_stride_b; p.xs[1] = a->x_stride_t;
+  p.ds[0] = a->dt_stride_b; p.ds[1] = a->dt_stride_t;
+  p.zs[0] = a->z_stride_b; p.zs[1] = a->z_stride_t;
+  p.bs[0] = a->b_stride_b; p.bs[1] = a->b_stride_t;
+  p.cs[0] = a->c_stride_b; p.cs[1] = a->c_stride_t;
   p.A = a->A; p.skip = a->skip; p.bias = a->dt_bias; p.h0 = a->h0;
   p.y = a->y; p.ht = a->ht; p.states = a->states;
   const int es = dtype_bytes(a->dtype);

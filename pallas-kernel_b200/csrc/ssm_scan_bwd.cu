@@ -547,7 +547,7 @@ TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream
   const size_t need = plan_bwd(p, a->workspace);
   if (need && (a->workspace == nullptr || a->workspace_bytes < need))
     return fail(TOPS_ERR_WORKSPACE, "ssm_scan_bwd: workspace smaller than tops_gla_ssm_scan_bwd_workspace_size()");
-  p.dout = a->dout; p.os[0] = a->dout_strides[0]; p.os[1] = a->dout_strides[1];
+  p.dout = a->dout; p.os[0] = a->dout_stride_b; p.os[1] = a->dout_stride_t;
   p.dht = a->dht; p.dx = a->dx; p.ddt = a->ddt; p.dz = a->dz; p.dh0 = a->dh0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int rc = empty_states(p, p.dht, p.dh0, st)) return rc;

@@ -99,14 +99,17 @@ class ScanArgs(C.Structure):
     _fields_ = [("B", C.c_int32), ("T", C.c_int32), ("D", C.c_int32), ("N", C.c_int32), ("G", C.c_int32),
                 ("S", C.c_int32), ("dtype", C.c_int32), ("softplus", C.c_int32), ("cu_seqlens", C.c_void_p),
                 ("x", C.c_void_p), ("dt", C.c_void_p), ("z", C.c_void_p), ("Bm", C.c_void_p), ("Cm", C.c_void_p),
-                ("x_strides", C.c_int64 * 2), ("dt_strides", C.c_int64 * 2), ("z_strides", C.c_int64 * 2),
-                ("b_strides", C.c_int64 * 2), ("c_strides", C.c_int64 * 2), ("A", C.c_void_p), ("skip", C.c_void_p),
+                ("x_stride_b", C.c_int64), ("x_stride_t", C.c_int64), ("dt_stride_b", C.c_int64),
+                ("dt_stride_t", C.c_int64), ("z_stride_b", C.c_int64), ("z_stride_t", C.c_int64),
+                ("b_stride_b", C.c_int64), ("b_stride_t", C.c_int64), ("c_stride_b", C.c_int64),
+                ("c_stride_t", C.c_int64), ("A", C.c_void_p), ("skip", C.c_void_p),
                 ("dt_bias", C.c_void_p), ("h0", C.c_void_p), ("y", C.c_void_p), ("ht", C.c_void_p),
                 ("states", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class ScanBwdArgs(C.Structure):
-    _fields_ = [("f", ScanArgs), ("dout", C.c_void_p), ("dout_strides", C.c_int64 * 2), ("dht", C.c_void_p),
+    _fields_ = [("f", ScanArgs), ("dout", C.c_void_p), ("dout_stride_b", C.c_int64), ("dout_stride_t", C.c_int64),
+                ("dht", C.c_void_p),
                 ("dx", C.c_void_p), ("ddt", C.c_void_p), ("dz", C.c_void_p), ("dB", C.c_void_p), ("dC", C.c_void_p),
                 ("dA", C.c_void_p), ("dskip", C.c_void_p), ("ddt_bias", C.c_void_p), ("dh0", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]

@@ -29,8 +29,8 @@ def _args(x, w, bias, state, y, final, act, N, cu):
 def _forward(x, w, bias, state, act, want_final, N, cu):
     x = _rows.rows(x)
     w, bias, state = (t if t is None else t.contiguous() for t in (w, bias, state))
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    final = torch.empty(N, x.shape[2], w.shape[1] - 1, dtype=x.dtype, device=x.device) if want_final else None
+    y = x.new_empty(x.shape)
+    final = x.new_empty((N, x.shape[2], w.shape[1] - 1)) if want_final else None
     _rows.launch("tops_gla_causal_conv_fwd", _args(x, w, bias, state, y, final, act, N, cu), x)
     return y, final
 
@@ -73,7 +73,7 @@ class _CausalConv(torch.autograd.Function):
         w, bias, state = (t if t is None else t.contiguous() for t in (w, bias, state))
         dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _rows.rows(dy.to(x.dtype))
         dfinal = None if dfinal is None else dfinal.to(x.dtype).contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = x.new_empty(x.shape)
         dw = torch.empty_like(w) if need[1] else None
         db = torch.empty_like(bias) if bias is not None and need[2] else None
         ds = torch.empty_like(state) if state is not None and need[3] else None
@@ -154,7 +154,7 @@ def causal_conv1d_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     x = _rows.rows(x)
     weight, bias = weight.contiguous(), None if bias is None else bias.contiguous()
     state, out = _rows.state_target(op, state, state_out, x, weight, bias)
-    y = torch.empty(B, D, dtype=x.dtype, device=x.device)
+    y = x.new_empty((B, D))
     a = _C.ConvArgs(B, 1, D, weight.shape[1], B, _C.dtype_code(x.dtype), _C.dtype_code(weight.dtype), _ACT[activation],
                     None, x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _C.ptr(bias), state.data_ptr(), y.data_ptr(),
                     out.data_ptr())

@@ -47,8 +47,7 @@ def _args(q, k, qw, kw, cos, sin, positions, eps, interleaved):
 def _forward(q, k, qw, kw, cos, sin, positions, eps, interleaved):
     q, k = _rows.rows(q), _rows.rows(k)
     qw, kw = (None if w is None else w.contiguous() for w in (qw, kw))
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
     a = _args(q, k, qw, kw, cos, sin, positions, eps, interleaved)
     a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
     _rows.launch("tops_gla_qk_norm_rotary_fwd", a, q)
@@ -69,8 +68,7 @@ class _QKNormRotary(torch.autograd.Function):
         q, k = _rows.rows(q), _rows.rows(k)
         qw, kw = (None if w is None else w.contiguous() for w in (qw, kw))
         dqo, dko = _rows.rows(dqo.to(q.dtype)), _rows.rows(dko.to(q.dtype))
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
         dqw, dkw = (torch.empty_like(w) if w is not None and need else None
                     for w, need in zip((qw, kw), ctx.needs_input_grad[2:4]))
         f = _args(q, k, qw, kw, cos, sin, positions, ctx.eps, ctx.interleaved)
@@ -101,7 +99,8 @@ def _check(op, q, k, q_weight, k_weight, cos, sin, positions):
     assert (cos is None) == (sin is None), f"{op}: cos and sin come together"
     if cos is None:
         return q_weight, k_weight, None, None, None
-    _rows.check_cuda(op, q, cos=cos, sin=sin, positions=positions)
+    if cos.get_device() != dev or sin.get_device() != dev or (positions is not None and positions.get_device() != dev):
+        _rows.check_cuda(op, q, cos=cos, sin=sin, positions=positions)
     R = 2 * cos.shape[-1]
     assert cos.dim() == 2 and cos.shape[0] > 0 and 0 < R <= K, \
         f"{op}: expected cos [P, R / 2] with R in 2..{K}, got {tuple(cos.shape)}"

@@ -20,17 +20,6 @@ __all__ = ["selective_scan", "selective_scan_step"]
 MAX_STATES = 64
 
 
-_S2 = _C.C.c_int64 * 2
-
-
-def _strides(t):
-    return _S2() if t is None else _S2(t.stride(0), t.stride(1))
-
-
-def _row_stride(t):
-    return _S2() if t is None else _S2(t.stride(0))
-
-
 def _f32(t):
     return t if t is None or t.dtype == torch.float32 else t.float()
 
@@ -38,9 +27,10 @@ def _f32(t):
 def _args(x, dt, A, Bm, Cm, D, z, bias, h0, softplus, S, cu):
     B, T, ch = x.shape
     G, N = Bm.shape[2:]
+    zb, zt = (0, 0) if z is None else z.stride()[:2]
     return _C.ScanArgs(B, T, ch, N, G, S, _C.dtype_code(x.dtype), softplus, _C.ptr(cu), x.data_ptr(), dt.data_ptr(),
-                       _C.ptr(z), Bm.data_ptr(), Cm.data_ptr(), _strides(x), _strides(dt), _strides(z), _strides(Bm),
-                       _strides(Cm), A.data_ptr(), _C.ptr(D), _C.ptr(bias), _C.ptr(h0), None, None, None, None, 0)
+                       _C.ptr(z), Bm.data_ptr(), Cm.data_ptr(), *x.stride()[:2], *dt.stride()[:2], zb, zt,
+                       *Bm.stride()[:2], *Cm.stride()[:2], A.data_ptr(), _C.ptr(D), _C.ptr(bias), _C.ptr(h0))
 
 
 def _dense(x, dt, A, Bm, Cm, D, z, bias, h0):
@@ -53,7 +43,7 @@ def _forward(x, dt, A, Bm, Cm, D, z, bias, h0, softplus, want_final, S, cu, save
     x, dt, A, Bm, Cm, D, z, bias, h0 = _dense(x, dt, A, Bm, Cm, D, z, bias, h0)
     a = _args(x, dt, A, Bm, Cm, D, z, bias, h0, softplus, S, cu)
     L = _C.lib()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     ht = torch.empty(S, x.shape[2], Bm.shape[3], dtype=torch.float32, device=x.device) if want_final else None
     states = None
     if save:
@@ -82,7 +72,7 @@ class _SelectiveScan(torch.autograd.Function):
         if dout is None and dht is None:
             return (None,) * 13
         x, dt, A, Bm, Cm, D, z, bias, h0 = _dense(*inputs)
-        new = lambda like: torch.empty(like.shape, dtype=like.dtype, device=x.device)  # noqa: E731
+        new = lambda like: like.new_empty(like.shape)  # noqa: E731
         dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dout is None else _rows.rows(dout.to(x.dtype))
         dht = None if dht is None else dht.float().contiguous()
         dx, ddt, dB, dC = new(x), new(dt), new(Bm), new(Cm)
@@ -93,8 +83,8 @@ class _SelectiveScan(torch.autograd.Function):
         dh0 = new(h0) if h0 is not None and need[8] else None
         f = _args(x, dt, A, Bm, Cm, D, z, bias, h0, ctx.softplus, ctx.S, cu)
         f.states = states.data_ptr()
-        a = _C.ScanBwdArgs(f, dout.data_ptr(), _strides(dout), _C.ptr(dht), dx.data_ptr(), ddt.data_ptr(), _C.ptr(dz),
-                           dB.data_ptr(), dC.data_ptr(), _C.ptr(dA), _C.ptr(dD), _C.ptr(dbias), _C.ptr(dh0), None, 0)
+        a = _C.ScanBwdArgs(f, dout.data_ptr(), *dout.stride()[:2], _C.ptr(dht), dx.data_ptr(), ddt.data_ptr(), _C.ptr(dz),
+                           dB.data_ptr(), dC.data_ptr(), _C.ptr(dA), _C.ptr(dD), _C.ptr(dbias), _C.ptr(dh0))
         ws = _rows.workspace(_C.lib().tops_gla_ssm_scan_bwd_workspace_size(a), x)
         a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
         _rows.launch("tops_gla_ssm_scan_bwd", a, x)
@@ -184,11 +174,11 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     A = _f32(A).contiguous()
     D, dt_bias = (None if t is None else _f32(t).contiguous() for t in (D, dt_bias))
     state, out = _rows.state_target(op, state, state_out, x, dt, A, B, C, D, z, dt_bias)
-    y = torch.empty(Bsz, ch, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     G, N = B.shape[1:]
-    s = _row_stride
     a = _C.ScanArgs(Bsz, 1, ch, N, G, Bsz, _C.dtype_code(x.dtype), int(dt_softplus), None, x.data_ptr(), dt.data_ptr(),
-                    _C.ptr(z), B.data_ptr(), C.data_ptr(), s(x), s(dt), s(z), s(B), s(C), A.data_ptr(), _C.ptr(D),
-                    _C.ptr(dt_bias), state.data_ptr(), y.data_ptr(), out.data_ptr(), None, None, 0)
+                    _C.ptr(z), B.data_ptr(), C.data_ptr(), x.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0),
+                    0, B.stride(0), 0, C.stride(0), 0, A.data_ptr(), _C.ptr(D), _C.ptr(dt_bias), state.data_ptr(),
+                    y.data_ptr(), out.data_ptr())
     _rows.launch("tops_gla_ssm_scan_step", a, x)
     return y, out
