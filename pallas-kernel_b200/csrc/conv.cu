@@ -4,8 +4,9 @@
 // newest input) or zeros.  Backward, with dp = dy y'(p):
 //   dx_s = sum_k w[:, W - 1 - k] dp_{s + k},   dw[:, j] = sum_t dp_t x_{t - W + 1 + j},   db = sum_t dp_t
 //
-// Nothing is reused but the W - 1 rows before a row, so HBM bounds it: a thread owns V channels
-// (16 bytes) and walks down a strip of rows with the window in registers.
+// Nothing is reused but the W - 1 rows before a row, so HBM bounds it: a thread owns V channels (16 bytes; 8 in the
+// backward, whose sums need the registers) and walks down a strip of rows with the window in registers.  B8 T4096 D2048
+// bf16: forward 52 us = 5.2 TB/s, backward 104 us = 3.9 TB/s, the latter bound by instruction issue.
 #include <algorithm>
 
 #include "rowtypes.cuh"
@@ -146,9 +147,22 @@ __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
   const int b = (int)(unit / p.strips);
   const int t0 = (int)(unit - (int64_t)b * p.strips) * p.strip;
   const int t1 = min(t0 + p.strip, p.T);
+  const T* x = static_cast<const T*>(p.x) + b * p.xb + d0;
+  constexpr int kAhead = 3, kSlots = R * (kAhead + 1);
+  __shared__ Raw<T, V> ring[V == 1 ? 1 : kSlots][128];
+  const int batches = (t1 - t0) / R;
+  auto ask = [&](int g) {
+    if (g < batches)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        copy_async<Raw<T, V>::B>(&ring[(g * R + r) % kSlots][threadIdx.x], x + (t0 + g * R + r) * p.xt);
+    copies_commit();
+  };
+  if constexpr (V > 1)  // the first rows are on their way while the weights and the sequence are looked up
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) ask(g);
   float w[W][V], bias[V];
   load_params<T, V, W>(p, d0, w, bias);
-  const T* x = static_cast<const T*>(p.x) + b * p.xb + d0;
   T* y = static_cast<T*>(p.y) + (int64_t)b * p.T * p.D + d0;
   SeqAt q = seq_of(p, b, t0);
   float win[W][V];  // rows t - W + 1 .. t
@@ -181,18 +195,6 @@ __global__ void __launch_bounds__(128) k_conv_fwd(const P p) {
     for (int t = t0; t < t1; ++t) row(t);
     return;
   } else {
-    constexpr int kAhead = 3, kSlots = R * (kAhead + 1);
-    __shared__ Raw<T, V> ring[kSlots][128];
-    const int batches = (t1 - t0) / R;
-    auto ask = [&](int g) {
-      if (g < batches)
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          copy_async<Raw<T, V>::B>(&ring[(g * R + r) % kSlots][threadIdx.x], x + (t0 + g * R + r) * p.xt);
-      copies_commit();
-    };
-#pragma unroll
-    for (int g = 0; g < kAhead; ++g) ask(g);
     for (int g = 0; g < batches; ++g) {
       ask(g + kAhead);
       copies_wait<kAhead>();
@@ -283,10 +285,10 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
   const int64_t unit = id / p.dv;
   const int d0 = (int)(id - unit * p.dv) * V;
   const int64_t nstrips = (int64_t)p.B * p.strips;
-  if (unit >= nstrips && (p.dstate == nullptr || unit - nstrips >= p.N)) return;
-  float w[W][V], bias[V];
-  load_params<T, V, W>(p, d0, w, bias);
   if (unit >= nstrips) {
+    if (p.dstate == nullptr || unit - nstrips >= p.N) return;
+    float w[W][V], bias[V];
+    load_params<T, V, W>(p, d0, w, bias);
     state_grad<T, V, W>(p, w, bias, (int)(unit - nstrips), d0);
     return;
   }
@@ -295,6 +297,24 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
   const int t1 = min(t0 + p.strip, p.T);
   const T* x = static_cast<const T*>(p.x) + b * p.xb + d0;
   const T* dy = static_cast<const T*>(p.dy) + b * p.gb + d0;
+  constexpr int kAhead = Raw<T, V>::B == 16 ? 1 : 3, kSlots = R * (kAhead + 1);  // 32 KB
+  __shared__ Raw<T, V> ring[2][V == 1 ? 1 : kSlots][128];
+  const int batches = (t1 - t0) / R;
+  auto ask = [&](int g) {
+    if (g < batches)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int t = t0 + g * R + r, at = (g * R + r) % kSlots;
+        copy_async<Raw<T, V>::B>(&ring[0][at][threadIdx.x], x + t * p.xt);
+        copy_async<Raw<T, V>::B>(&ring[1][at][threadIdx.x], dy + t * p.gt);
+      }
+    copies_commit();
+  };
+  if constexpr (V > 1)
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) ask(g);
+  float w[W][V], bias[V];
+  load_params<T, V, W>(p, d0, w, bias);
   T* dx = static_cast<T*>(p.dx) + (int64_t)b * p.T * p.D + d0;
   SeqAt q = seq_of(p, b, t0);
   float win[W][V], acc[W][V], dw[W][V], db[V];  // acc[k]: dx of row t - k so far
@@ -353,21 +373,6 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const P p) {
   if constexpr (V == 1) {
     for (int t = t0; t < stop; ++t) row(t);
   } else {
-    constexpr int kAhead = Raw<T, V>::B == 16 ? 1 : 3, kSlots = R * (kAhead + 1);  // 32 KB
-    __shared__ Raw<T, V> ring[2][kSlots][128];
-    const int batches = (t1 - t0) / R;
-    auto ask = [&](int g) {
-      if (g < batches)
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int t = t0 + g * R + r, at = (g * R + r) % kSlots;
-          copy_async<Raw<T, V>::B>(&ring[0][at][threadIdx.x], x + t * p.xt);
-          copy_async<Raw<T, V>::B>(&ring[1][at][threadIdx.x], dy + t * p.gt);
-        }
-      copies_commit();
-    };
-#pragma unroll
-    for (int g = 0; g < kAhead; ++g) ask(g);
     for (int g = 0; g < batches; ++g) {
       ask(g + kAhead);
       copies_wait<kAhead>();
@@ -539,12 +544,15 @@ P params(const tops_gla_conv_args* a) {
 // rarely, short ones give every SM threads to hide the loads with.
 void split(P& p, int v, int64_t threads_wanted, int most) {
   p.dv = p.D / v;
-  const int64_t rows = std::max<int64_t>(1, (int64_t)p.B * p.T * p.dv / threads_wanted);
+  const int64_t rows = ((int64_t)p.B * p.T * p.dv + threads_wanted - 1) / threads_wanted;
   p.strip = (int)std::min<int64_t>(most, std::max<int64_t>(8, rows));
   p.strips = (p.T + p.strip - 1) / p.strip;
 }
 
-constexpr int64_t kFwdThreads = 148 * 1536, kBwdThreads = 148 * 768;
+// Four blocks of 128 threads fill an SM's registers: strips that make one wave of them (forward) or two (backward), as
+// far as the cap lets them (23 packed prompts of 9973 rows: 22 -> 18 us against strips of 8; backward B8 T4096 D2048: 1024
+// threads an SM 108 us, 512: 114, 1536: 116).
+constexpr int64_t kFwdThreads = 148 * 512, kBwdThreads = 148 * 1024;
 
 }  // namespace conv
 }  // namespace tops

@@ -89,7 +89,7 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src) {
     copy_async<16>(dst, src);
     copy_async<BYTES - 16>(static_cast<char*>(dst) + 16, static_cast<const char*>(src) + 16);
   } else if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(a), "l"(src) : "memory");
+  else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(a), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int AHEAD>
