@@ -11,7 +11,6 @@ namespace tops {
 template <typename T, int V>
 struct Vx {
   static constexpr int BYTES = V * (int)sizeof(T);
-  static constexpr int UNIT = BYTES >= 16 ? 16 : BYTES;  // one access
   static __device__ __forceinline__ void load(const T* p, float (&r)[V]) {
     alignas(16) T raw[V];
     load_raw(p, raw);
@@ -187,13 +186,6 @@ __device__ __forceinline__ SeqAt seq_at(const int32_t* __restrict__ cu, int N, i
   SeqAt q{lo, max(__ldg(cu + lo), 0), min(__ldg(cu + lo + 1), T)};
   if (t < q.s || t >= q.e) q.n = -1;
   return q;
-}
-
-inline int sm_count() {
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
 }
 
 inline bool dtype_known(int d) { return d == TOPS_F32 || d == TOPS_BF16 || d == TOPS_F16; }

@@ -51,9 +51,11 @@ constexpr size_t bwd_smem() {
          ((kBwdThreads / LN) * 6 + 2 * Order<LN, NT>::COPIES * LN * NT + kBwdThreads / 32 * 2 * LN * NT);
 }
 
-// One segment, tile by tile from its end.  The states of 8 rows at a time are computed again from the saved state
-// before them and kept in registers with their decays; what the tile's outputs need of the inputs stays packed as it
-// came (a tile's worth of fp32 copies spilled), the rest is read back from shared memory.
+// One segment, tile by tile from its end.  The states of kBwdPart rows at a time are computed again from the saved state
+// before them and kept in registers with their decays (eight rows spilled: 1088 against 1004 us); what the tile's outputs
+// need of the inputs stays packed as it came, the rest is read back from shared memory.  B4 T2048 D4096 N16 bf16: 925 us
+// at 256 blocks, 800 us for the same work in many more blocks; bound by instruction issue and the shared-memory pipe
+// (33 instructions and 0.28 wavefronts an element, of which the folds are 10 and 0.08).
 template <typename T, int LN, int NT, bool VAR>
 __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
   constexpr int TS = kBwdRows, HALF = kBwdPart, DB = kBwdThreads / LN, NP = LN * NT, QC = DB / 4, NH = NT / 2;
