@@ -18,6 +18,7 @@ __global__ void __launch_bounds__(kFwdThreads) k_scan_fwd(const P p) {
   __shared__ __align__(16) float2 su[TS][DB];
   __shared__ __align__(16) float sb[TS][NP], sc[TS][NP], sy[TS][DB];
   __shared__ int sflag[TS], sseq[TS];
+  __shared__ unsigned smark;
   const int tid = threadIdx.x, lane = tid & 31, nl = lane % LN, b = blockIdx.y, k = blockIdx.z;
   const int rep = p.D / p.G, nblk = (rep + DB - 1) / DB, grp = blockIdx.x / nblk;
   const int c0 = (blockIdx.x - grp * nblk) * DB;                   // first channel of the block in its group
@@ -79,14 +80,18 @@ __global__ void __launch_bounds__(kFwdThreads) k_scan_fwd(const P p) {
   fetch(t_first);
   int broken = 0;
   for (int t0 = t_first; t0 < t_end; t0 += TS) {
-    bool flagged = false;  // a row of the tile begins or ends a sequence, or belongs to none
+    unsigned marks = 0;  // a bit for every row of the tile that begins or ends a sequence, or belongs to none
     if (VAR) {
+      static_assert(TS == 32, "one warp marks a tile's rows");
       if (tid < TS) {
         sflag[tid] = flag;
         sseq[tid] = seq;
+        marks = __ballot_sync(0xffffffffu, flag);
+        if (tid == 0) smark = marks;
+        if (SUM) broken |= __ballot_sync(0xffffffffu, flag & (kFirst | kNone));
       }
-      flagged = __syncthreads_or(flag);
-      if (SUM && flagged) broken |= __syncthreads_or(flag & (kFirst | kNone));
+      __syncthreads();
+      marks = smark;
     }
     Quad<T> xc[QN], zc[QN];
 #pragma unroll
@@ -126,73 +131,73 @@ __global__ void __launch_bounds__(kFwdThreads) k_scan_fwd(const P p) {
     const int rows = min(TS, t_end - t0);
 
     auto save = [&](int r) {
+      static_assert(CK % RG == 0, "states are saved where a group of rows begins");
       if (!SUM && p.states != nullptr && on && (r & (CK - 1)) == 0) {
         const int nck = (p.T + CK - 1) / CK;
         states_store<NT>(p.states + (((int64_t)b * nck + (t0 + r) / CK) * p.D + d) * p.N, n0, p.N, h);
       }
     };
-    if (VAR && flagged) {  // row by row: few tiles of a packed batch
 #pragma unroll 1
-      for (int r = 0; r < rows; ++r) {
-        save(r);
-        const int f = sflag[r];
-        if (f & (kFirst | kNone)) {
-#pragma unroll
-          for (int j = 0; j < NH; ++j) h[j] = dup(0.f);
-          if ((f & kFirst) && p.h0 && on) states_load<NT>(p.h0 + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, h);
-        }
-        float2 Bv[NH], Cv[NH], acc = dup(0.f);
-        pairs_load<NT>(&sb[r][n0], Bv);
-        if (!SUM) pairs_load<NT>(&sc[r][n0], Cv);
-        const float2 q = su[r][cb];
-        if (SUM) dsum += q.x;
-#pragma unroll
-        for (int j = 0; j < NH; ++j) {
-          h[j] = fma2(decay2(q.x, A[j]), h[j], mul2(dup(q.y), Bv[j]));
-          if (!SUM) acc = j ? fma2(Cv[j], h[j], acc) : mul2(Cv[j], h[j]);
-        }
-        if (!SUM) {
-          float y[1] = {acc.x + acc.y};
-          fold<1, LN, 1>(y, lane);
-          sy[r][cb] = y[0];
-          if ((f & kLast) && p.ht && on) states_store<NT>(p.ht + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, h);
-        }
-      }
-    } else {
+    for (int r0 = 0; r0 < rows; r0 += RG) {  // rows at t_end and beyond: delta = 0, nothing moves
+      save(r0);
+      if (VAR && (marks >> r0 & ((1u << RG) - 1))) {  // one by one: few rows of a packed batch
 #pragma unroll 1
-      for (int r0 = 0; r0 < rows; r0 += RG) {  // rows at t_end and beyond: delta = 0, nothing moves
-        save(r0);
-        // the decays and inputs of all rows first: nothing of them waits for a state
-        float2 a[RG][NH], ub[RG][NH];
+        for (int r = r0; r < min(r0 + RG, rows); ++r) {
+          const int f = sflag[r];
+          if (f & (kFirst | kNone)) {
 #pragma unroll
-        for (int rr = 0; rr < RG; ++rr) {
-          float2 Bv[NH];
-          pairs_load<NT>(&sb[r0 + rr][n0], Bv);
-          const float2 q = su[r0 + rr][cb];
+            for (int j = 0; j < NH; ++j) h[j] = dup(0.f);
+            if ((f & kFirst) && p.h0 && on) states_load<NT>(p.h0 + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, h);
+          }
+          float2 Bv[NH], Cv[NH], acc = dup(0.f);
+          pairs_load<NT>(&sb[r][n0], Bv);
+          if (!SUM) pairs_load<NT>(&sc[r][n0], Cv);
+          const float2 q = su[r][cb];
           if (SUM) dsum += q.x;
 #pragma unroll
           for (int j = 0; j < NH; ++j) {
-            a[rr][j] = decay2(q.x, A[j]);
-            ub[rr][j] = mul2(dup(q.y), Bv[j]);
-          }
-        }
-        float ys[RG];
-#pragma unroll
-        for (int rr = 0; rr < RG; ++rr) {
-          float2 Cv[NH], acc = dup(0.f);
-          if (!SUM) pairs_load<NT>(&sc[r0 + rr][n0], Cv);
-#pragma unroll
-          for (int j = 0; j < NH; ++j) {
-            h[j] = fma2(a[rr][j], h[j], ub[rr][j]);
+            h[j] = fma2(decay2(q.x, A[j]), h[j], mul2(dup(q.y), Bv[j]));
             if (!SUM) acc = j ? fma2(Cv[j], h[j], acc) : mul2(Cv[j], h[j]);
           }
-          if (!SUM) ys[rr] = acc.x + acc.y;
+          if (!SUM) {
+            float y[1] = {acc.x + acc.y};
+            fold<1, LN, 1>(y, lane);
+            sy[r][cb] = y[0];
+            if ((f & kLast) && p.ht && on) states_store<NT>(p.ht + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, h);
+          }
         }
-        if (!SUM) {
-          const int at = fold<RG, LN, 1>(ys, lane);
+        continue;
+      }
+      // the decays and inputs of all rows first: nothing of them waits for a state
+      float2 a[RG][NH], ub[RG][NH];
 #pragma unroll
-          for (int i = 0; i < (RG > LN ? RG / LN : 1); ++i) sy[r0 + at + i][cb] = ys[i];
+      for (int rr = 0; rr < RG; ++rr) {
+        float2 Bv[NH];
+        pairs_load<NT>(&sb[r0 + rr][n0], Bv);
+        const float2 q = su[r0 + rr][cb];
+        if (SUM) dsum += q.x;
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+          a[rr][j] = decay2(q.x, A[j]);
+          ub[rr][j] = mul2(dup(q.y), Bv[j]);
         }
+      }
+      float ys[RG];
+#pragma unroll
+      for (int rr = 0; rr < RG; ++rr) {
+        float2 Cv[NH], acc = dup(0.f);
+        if (!SUM) pairs_load<NT>(&sc[r0 + rr][n0], Cv);
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+          h[j] = fma2(a[rr][j], h[j], ub[rr][j]);
+          if (!SUM) acc = j ? fma2(Cv[j], h[j], acc) : mul2(Cv[j], h[j]);
+        }
+        if (!SUM) ys[rr] = acc.x + acc.y;
+      }
+      if (!SUM) {
+        const int at = fold<RG, LN, 1>(ys, lane);
+#pragma unroll
+        for (int i = 0; i < (RG > LN ? RG / LN : 1); ++i) sy[r0 + at + i][cb] = ys[i];
       }
     }
     __syncthreads();
@@ -327,7 +332,7 @@ __global__ void __launch_bounds__(256) k_scan_step(const P p, int R) {
 }
 
 size_t plan_fwd(P& p, void* ws) {
-  split(p, blocks_of(p, kFwdThreads / lanes_of(p.N)), kFwdBlocks);
+  split(p, blocks_of(p, kFwdThreads / lanes_of(p.N)), kFwdBlocks, p.cu ? 5 : 4);
   Carve c{static_cast<char*>(ws)};
   return carve_segments(p, c);
 }

@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(256) k_scan_fold(const P p, int64_t bc_blocks,
 
 size_t plan_bwd(P& p, void* ws) {
   p.parts = blocks_of(p, kBwdThreads / lanes_of(p.N)) / p.G;
-  split(p, p.parts * p.G, kBwdBlocks);
+  split(p, p.parts * p.G, kBwdBlocks, 2);
   Carve c{static_cast<char*>(ws)};
   p.pbc = c.take((size_t)p.G * p.parts * p.B * p.T * 2 * p.N);
   p.pa = c.take((size_t)p.B * p.nseg * p.D * p.N);

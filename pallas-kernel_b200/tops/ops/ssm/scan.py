@@ -130,7 +130,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     """Selective state space scan over time -> ``(out, final_state or None)``.
 
     Args:
-        x, dt: [B, T, D] fp32, bf16 or fp16; z: [B, T, D] output gate (optional), x's dtype
+        x, dt: [B, T, D] fp32, bf16 or fp16; z: [B, T, D] output gate (optional); dt, z, B and C in x's dtype
         A: [D, N], N up to 64; B, C: [B, T, N], or [B, T, G, N] shared by the D / G channels of a group
         D: [D] skip weight; dt_bias: [D]; dt_softplus: delta = softplus(dt + dt_bias)
         initial_state: [S, D, N]; output_final_state: return the final state [S, D, N], fp32
