@@ -381,13 +381,15 @@ __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
 }
 
 // The backward's first pass over a segment: the gradient that leaves it with nothing coming in, and the sum of delta.
+// As the forward's: loads a tile ahead, the decays and inputs of eight rows before the rows themselves.
 template <typename T, int LN, int NT, bool VAR>
 __global__ void __launch_bounds__(128) k_scan_bwd_sum(const P p) {
   constexpr int TS = 32, DB = 128 / LN, NP = LN * NT, QC = DB / 4, RPP = 128 / QC, QN = RPP >= TS ? 1 : TS / RPP;
-  constexpr int NH = NT / 2, BQ = TS * NP / 4, BN = (BQ + 127) / 128;
+  constexpr int NH = NT / 2, BQ = TS * NP / 4, BN = (BQ + 127) / 128, RG = 8;
   __shared__ __align__(16) float2 su[TS][DB];  // delta, dy
   __shared__ __align__(16) float sc[TS][NP];
   __shared__ int sflag[TS], sseq[TS];
+  __shared__ unsigned smark;
   const int tid = threadIdx.x, lane = tid & 31, nl = lane % LN, b = blockIdx.y, k = blockIdx.z + 1;  // segment 0 passes nothing on
   const int rep = p.D / p.G, nblk = (rep + DB - 1) / DB, grp = blockIdx.x / nblk;
   const int c0 = (blockIdx.x - grp * nblk) * DB, cb = tid / 32 * (32 / LN) + lane / LN, n0 = nl * NT;
@@ -408,38 +410,56 @@ __global__ void __launch_bounds__(128) k_scan_bwd_sum(const P p) {
   float bias[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) bias[i] = p.bias && i < valid ? p.bias[qd + i] : 0.f;
-  int broken = 0;
-  const int last = t_first + (t_end - t_first - 1) / TS * TS;
-  for (int t0 = last; t0 >= t_first; t0 -= TS) {
-    int flag = 0, seq = 0;
-    if (VAR) {
-      if (tid < TS) {
-        flag = t0 + tid < t_end ? row_flags(p, t0 + tid, seq) : 0;
-        sflag[tid] = flag;
-        sseq[tid] = seq;
-      }
-      broken |= __syncthreads_or(flag & (kLast | kNone));
-    }
+  Quad<T> dr[QN], gr[QN], zr[QN], cr[BN];
+  int flag = 0, seq = 0;
+  auto fetch = [&](int t0) {
 #pragma unroll
     for (int j = 0; j < QN; ++j) {
       const int row = qr + j * RPP, t = t0 + row;
+      const int v = (row < TS && t < t_end) ? valid : 0;
+      quad_load<T>(static_cast<const T*>(p.dt) + b * p.ds[0] + t * p.ds[1] + qd, p.vd, v, dr[j]);
+      quad_load<T>(static_cast<const T*>(p.dout) + b * p.os[0] + t * p.os[1] + qd, p.vo, v, gr[j]);
+      quad_load<T>(static_cast<const T*>(p.z) + b * p.zs[0] + t * p.zs[1] + qd, p.vz, p.z ? v : 0, zr[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < BN; ++j) {
+      const int q = tid + j * 128, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4;
+      const int v = (q < BQ && t0 + row < t_end) ? min(max(p.N - n, 0), 4) : 0;
+      quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + (t0 + row) * p.cs[1] + grp * p.N + n, p.vc, v, cr[j]);
+    }
+    if (VAR && tid < TS) flag = t0 + tid < t_end ? row_flags(p, t0 + tid, seq) : 0;
+  };
+  unsigned broken = 0;
+  const int last = t_end > t_first ? t_first + (t_end - t_first - 1) / TS * TS : t_first - TS;
+  if (last >= t_first) fetch(last);
+  for (int t0 = last; t0 >= t_first; t0 -= TS) {
+    unsigned marks = 0;  // a bit for every row of the tile that begins or ends a sequence, or belongs to none
+    if (VAR) {
+      if (tid < TS) {
+        sflag[tid] = flag;
+        sseq[tid] = seq;
+        marks = __ballot_sync(0xffffffffu, flag);
+        if (tid == 0) smark = marks;
+        broken |= __ballot_sync(0xffffffffu, flag & (kLast | kNone));
+      }
+      __syncthreads();
+      marks = smark;
+    }
+#pragma unroll
+    for (int j = 0; j < QN; ++j) {
+      const int row = qr + j * RPP;
       if (row >= TS) continue;
-      const bool gone = t >= t_end || (VAR && (sflag[row] & kNone));
-      Quad<T> dr, gr, zr;
-      const int v = gone ? 0 : valid;
-      quad_load<T>(static_cast<const T*>(p.dt) + b * p.ds[0] + t * p.ds[1] + qd, p.vd, v, dr);
-      quad_load<T>(static_cast<const T*>(p.dout) + b * p.os[0] + t * p.os[1] + qd, p.vo, v, gr);
-      quad_load<T>(static_cast<const T*>(p.z) + b * p.zs[0] + t * p.zs[1] + qd, p.vz, p.z ? v : 0, zr);
+      const bool gone = t0 + row >= t_end || (VAR && (sflag[row] & kNone));
       float f[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float z = zr.get(i);
-        const float dy = p.z ? gr.get(i) * z * fast_sigmoid(z) : gr.get(i);
+        const float z = zr[j].get(i);
+        const float dy = p.z ? gr[j].get(i) * z * fast_sigmoid(z) : gr[j].get(i);
         f[2 * i + 1] = gone ? 0.f : dy;
       }
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        float2 dl = make_float2(dr.get(i) + bias[i], dr.get(i + 1) + bias[i + 1]);
+        float2 dl = make_float2(dr[j].get(i) + bias[i], dr[j].get(i + 1) + bias[i + 1]);
         if (p.softplus) dl = softplus2(dl);
         f[2 * i] = gone ? 0.f : dl.x;
         f[2 * i + 2] = gone ? 0.f : dl.y;
@@ -451,26 +471,54 @@ __global__ void __launch_bounds__(128) k_scan_bwd_sum(const P p) {
     for (int j = 0; j < BN; ++j) {
       const int q = tid + j * 128, row = q / (NP / 4), n = (q - row * (NP / 4)) * 4;
       if (q >= BQ) continue;
-      const bool gone = t0 + row >= t_end || (VAR && (sflag[row] & kNone));
-      Quad<T> cr;
-      quad_load<T>(static_cast<const T*>(p.cm) + b * p.cs[0] + (t0 + row) * p.cs[1] + grp * p.N + n, p.vc,
-                   gone ? 0 : min(max(p.N - n, 0), 4), cr);
-      *reinterpret_cast<float4*>(&sc[row][n]) =
-          make_float4(cr.get(0), cr.get(1), cr.get(2), cr.get(3));
+      const bool none = VAR && (sflag[row] & kNone);
+      float fc[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fc[i] = none ? 0.f : cr[j].get(i);
+      *reinterpret_cast<float4*>(&sc[row][n]) = make_float4(fc[0], fc[1], fc[2], fc[3]);
     }
     __syncthreads();
-    for (int r = min(TS, t_end - t0) - 1; r >= 0; --r) {
-      if (VAR && (sflag[r] & (kLast | kNone))) {
+    if (t0 > t_first) fetch(t0 - TS);
+#pragma unroll 1
+    for (int r0 = (min(TS, t_end - t0) - 1) / RG * RG; r0 >= 0; r0 -= RG) {  // rows at t_end and beyond: nothing moves
+      if (VAR && (marks >> r0 & ((1u << RG) - 1))) {
+#pragma unroll 1
+        for (int r = min(r0 + RG, t_end - t0) - 1; r >= r0; --r) {
+          const int f = sflag[r];
+          if (f & (kLast | kNone)) {
 #pragma unroll
-        for (int j = 0; j < NH; ++j) g[j] = dup(0.f);
-        if ((sflag[r] & kLast) && p.dht && on) states_load<NT>(p.dht + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, g);
+            for (int j = 0; j < NH; ++j) g[j] = dup(0.f);
+            if ((f & kLast) && p.dht && on) states_load<NT>(p.dht + ((int64_t)sseq[r] * p.D + d) * p.N, n0, p.N, g);
+          }
+          float2 Cv[NH];
+          pairs_load<NT>(&sc[r][n0], Cv);
+          const float2 q = su[r][cb];
+#pragma unroll
+          for (int j = 0; j < NH; ++j) g[j] = mul2(decay2(q.x, A[j]), fma2(Cv[j], dup(q.y), g[j]));
+          dsum += q.x;
+        }
+        continue;
       }
-      float2 Cv[NH];
-      pairs_load<NT>(&sc[r][n0], Cv);
-      const float2 q = su[r][cb];
+      float2 a[RG][NH], in[RG][NH];
 #pragma unroll
-      for (int j = 0; j < NH; ++j) g[j] = mul2(decay2(q.x, A[j]), fma2(Cv[j], dup(q.y), g[j]));
-      dsum += q.x;
+      for (int r = 0; r < RG; ++r) {
+        float2 Cv[NH];
+        pairs_load<NT>(&sc[r0 + r][n0], Cv);
+        const float2 q = su[r0 + r][cb];
+        dsum += q.x;
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+          a[r][j] = decay2(q.x, A[j]);
+          in[r][j] = mul2(Cv[j], dup(q.y));
+        }
+      }
+#pragma unroll
+      for (int r = RG - 1; r >= 0; --r)
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+          const float2 s = make_float2(in[r][j].x + g[j].x, in[r][j].y + g[j].y);
+          g[j] = mul2(a[r][j], s);
+        }
     }
     __syncthreads();
   }
