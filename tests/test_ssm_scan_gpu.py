@@ -192,6 +192,25 @@ def test_scan_steps_continue_a_prompt(dt, B, ch, N, G):
     close("state", s, *r["ht"], n)
 
 
+def test_scan_step_of_many_rows_is_its_parts():
+    """So many rows that a thread takes eight of them: the same bits as from calls of few rows."""
+    from tops.ops.ssm import selective_scan_step
+    B, ch, N = 157, 2048, 16
+    t, _, _ = _mk(19, B, 1, ch, N, 1, torch.bfloat16, B)
+    c = {k: v.cuda() for k, v in t.items()}
+
+    def step(a, b):
+        return selective_scan_step(c["x"][a:b, 0], c["dt"][a:b, 0], c["A"], c["B"][a:b, 0], c["C"][a:b, 0], c["h0"][a:b],
+                                   D=c["D"], z=c["z"][a:b, 0], dt_bias=c["bias"], dt_softplus=True)
+
+    y, s = step(0, B)
+    parts = [step(a, min(a + 40, B)) for a in range(0, B, 40)]
+    assert torch.equal(y, torch.cat([p[0] for p in parts])) and torch.equal(s, torch.cat([p[1] for p in parts]))
+    r = scan_ref(*(_dbl(t[k][-2:]) if k in ("x", "dt", "B", "C", "z", "h0") else _dbl(t[k]) for k in NAMES), True, None)
+    close("y", y[-2:], r["out"][0][:, 0], r["out"][1][:, 0], _roundings(1, N, ch, 1))
+    close("s", s[-2:], *r["ht"], _roundings(1, N, ch, 1))
+
+
 def test_scan_step_without_optional_parts():
     from tops.ops.ssm import selective_scan_step
     t, _, _ = _mk(13, 4, 1, 32, 16, 1, torch.float32, 4, False, False, False)
