@@ -3,8 +3,27 @@
 from __future__ import annotations
 
 import torch
+from torch._C import _is_tracing, _len_torch_dispatch_stack
+from torch._C._functorch import peek_interpreter_stack
+from torch.autograd import forward_ad
 
 from . import _C
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether forward-mode differentiation goes through one of the tensors."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def plain(*tensors) -> bool:
+    """Whether the call is eager and on tensors of its own memory.  A kernel reads and writes through addresses:
+    ``torch.jit.trace``, ``torch.func``, forward mode, dispatch modes (``make_fx``, fake tensors, FLOP counts) and
+    tensor subclasses see none of it, so a module whose torch form they followed goes that way there."""
+    if _is_tracing() or _len_torch_dispatch_stack() or peek_interpreter_stack() is not None:
+        return False
+    return not has_tangent(*tensors) and all(
+        t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
 
 
 def check_cuda(op: str, first: torch.Tensor, **others) -> None:

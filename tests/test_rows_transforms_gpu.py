@@ -1,0 +1,125 @@
+"""ShortConvolution, causal_conv1d, selective_scan and qk_norm_rotary where something else than plain eager autograd
+looks at the call: tracing, forward mode, torch.func, batched and second gradients, fake tensors, dispatch modes."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+from torch.func import functional_call
+
+from _rows_ref import U32, close, conv_ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _no_tf32():
+    """torch's conv1d in full fp32, so that one bound holds for both ways."""
+    with torch.backends.cudnn.flags(enabled=True, benchmark=False, deterministic=True, allow_tf32=False):
+        yield
+
+
+def _pair(bias=True, seed=1, D=24):
+    """The module on the GPU and the same in 64 bits on the CPU (torch's conv1d)."""
+    from tops.modules import ShortConvolution
+    torch.manual_seed(seed)
+    g = ShortConvolution(D, 4, bias=bias)
+    if bias:
+        g.bias.data.normal_()
+    c = ShortConvolution(D, 4, bias=bias).double()
+    c.load_state_dict(g.state_dict())
+    return g.cuda(), c
+
+
+def _near(name, got, want, size=1.0, roundings=64):
+    """|got - want| <= roundings * 2^-24 * (largest |want| + size): W products and sums, the activation and its first
+    derivatives are at most 48 roundings of terms no larger than `size` (here W |w| |x| |dy|, below)."""
+    g, w = got.detach().double().cpu(), want.detach().double().cpu()
+    assert g.shape == w.shape, f"{name}: {tuple(g.shape)} {tuple(w.shape)}"
+    assert torch.isfinite(g).all(), f"{name}: non-finite values"
+    err = (g - w).abs().max().item()
+    assert err <= roundings * U32 * (w.abs().max().item() + size), f"{name}: {err:.2e}"
+
+
+SIZE = 4 * 0.5 * 5.0 * 5.0  # taps, |w| <= 1/2, normal inputs and tangents below 5
+
+
+def test_traced_short_convolution():
+    class Whole(torch.nn.Module):
+        def __init__(self, m):
+            super().__init__()
+            self.m = m
+
+        def forward(self, t):
+            return self.m(t, None, True)
+
+    g, c = _pair()
+    x, x2 = torch.randn(2, 13, 24), torch.randn(2, 13, 24)
+    with torch.no_grad():
+        tr = torch.jit.trace(Whole(g), x.cuda(), check_trace=False)
+        y, cache = tr(x2.cuda())
+    want, wc = c(x2.double(), None, True)
+    _near("y", y, want, SIZE)
+    assert torch.equal(cache.double().cpu(), wc)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_short_convolution(grad):
+    g, c = _pair()
+    x, t, tw, cache, tc = (torch.randn(*s) for s in ((2, 13, 24), (2, 13, 24), (24, 1, 4), (2, 24, 3), (2, 24, 3)))
+
+    def go(m, cast):
+        with torch.set_grad_enabled(grad), fwAD.dual_level():
+            dual = lambda p, q: fwAD.make_dual(cast(p), cast(q))  # noqa: E731
+            w = fwAD.make_dual(m.weight.detach(), cast(tw))
+            y, _ = functional_call(m, {"weight": w, "bias": m.bias.detach()}, (dual(x, t), dual(cache, tc)))
+            only_w, _ = functional_call(m, {"weight": w, "bias": m.bias.detach()}, (cast(x),))
+            return [v for r in (y, only_w) for v in fwAD.unpack_dual(r)]
+
+    for i, (a, b) in enumerate(zip(go(g, lambda v: v.cuda()), go(c, lambda v: v.double()))):
+        assert a is not None, f"output {i}: no tangent"
+        _near(str(i), a, b, 4 * SIZE)
+
+
+def test_short_convolution_under_torch_func():
+    g, c = _pair()
+    x, t = torch.randn(3, 2, 9, 24), torch.randn(2, 9, 24)
+
+    def run(m, cast):
+        ps = {k: v.detach() for k, v in m.named_parameters()}
+        f = lambda p, v: functional_call(m, p, (v,))[0]  # noqa: E731
+        loss = lambda p, v: f(p, v).square().sum()  # noqa: E731
+        X = cast(x)
+        return {"grad": torch.func.grad(loss)(ps, X[0])["weight"], "vmap": torch.vmap(lambda v: f(ps, v))(X),
+                "per sample": torch.vmap(torch.func.grad(loss), (None, 0))(ps, X)["bias"],
+                "jvp": torch.func.jvp(lambda v: f(ps, v), (X[0],), (cast(t),))[1],
+                "hvp": torch.func.jvp(torch.func.grad(lambda v: loss(ps, v)), (X[0],), (cast(t),))[1]}
+
+    got, want = run(g, lambda v: v.cuda()), run(c, lambda v: v.double())
+    for k in want:
+        _near(k, got[k], want[k], 20 * SIZE, 256)  # gradients of a square: one product more, sums of 18 rows
+
+
+def test_short_convolution_sees_modes_and_compilers():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    g, c = _pair()
+    x, x2 = torch.randn(2, 13, 24), torch.randn(2, 13, 24)
+    with torch.no_grad():
+        gm = make_fx(lambda t: g(t)[0])(x.cuda())
+        _near("make_fx", gm(x2.cuda()), c(x2.double())[0], SIZE)
+        with FlopCounterMode(display=False) as f:
+            g(x.cuda())
+        assert f.get_total_flops() > 0
+        with torch._subclasses.FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            y, s = g(mode.from_tensor(x.cuda()), None, True)
+        assert y.shape == (2, 13, 24) and s.shape == (2, 24, 3)
+        _near("compiled", torch.compile(g, backend="eager")(x2.cuda())[0], c(x2.double())[0], SIZE)
+
+
+def test_eager_short_convolution():
+    """Eager calls stay on the kernel: its values within its own, tighter bound."""
+    g, c = _pair(bias=False, D=40)
+    x = torch.randn(2, 30, 40)
+    r = conv_ref(x.double(), c.weight.detach().squeeze(1), None, None, 1, None)
+    close("y", g(x.cuda())[0], *r["y"], 24)
