@@ -3,7 +3,7 @@
 from __future__ import annotations
 
 import torch
-from torch._C import _is_tracing, _len_torch_dispatch_stack
+from torch._C import _get_dispatch_mode, _has_storage, _is_tracing, _len_torch_dispatch_stack, _TorchDispatchModeKey
 from torch._C._functorch import peek_interpreter_stack
 from torch.autograd import forward_ad
 
@@ -24,6 +24,27 @@ def plain(*tensors) -> bool:
         return False
     return not has_tangent(*tensors) and all(
         t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
+
+
+def eager_only(op: str, *tensors) -> None:
+    """Refuses what a kernel's launch would silently fall out of: a recording would hold an empty output, a tangent
+    would be dropped, a batch dimension or a fake tensor has no memory of its own."""
+    if _is_tracing() or (_len_torch_dispatch_stack() and _get_dispatch_mode(_TorchDispatchModeKey.PROXY) is not None):
+        raise RuntimeError(f"{op} cannot be traced (its kernel writes through addresses, which a trace does not record)")
+    if peek_interpreter_stack() is not None:
+        raise RuntimeError(f"{op} cannot be transformed by torch.func (vmap, grad, jvp)")
+    if _len_torch_dispatch_stack() and _get_dispatch_mode(_TorchDispatchModeKey.FAKE) is not None:
+        raise RuntimeError(f"{op} cannot run on fake tensors: there is no memory behind them")
+    if has_tangent(*tensors):
+        raise RuntimeError(f"{op} has no forward-mode derivative: a tensor carries a tangent")
+
+
+def eager_grads(op: str, *grads) -> None:
+    """``eager_only`` for the gradients that a backward is given (it may run on another thread than a transform)."""
+    eager_only(op, *grads)
+    for g in grads:
+        if g is not None and not _has_storage(g):
+            raise RuntimeError(f"{op} has no gradient for a batch of them (is_grads_batched, torch.func)")
 
 
 def check_cuda(op: str, first: torch.Tensor, **others) -> None:

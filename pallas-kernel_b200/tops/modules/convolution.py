@@ -124,9 +124,11 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
         cu_seqlens: [N + 1] offsets of N sequences packed along T (B must be 1).  Offsets on the GPU are
             not read by the host (capturable); rows behind the last sequence give zeros.
     Gradients flow to x, weight, bias and initial_state, also from the final state; where sequences
-    are not packed they can be differentiated again.
+    are not packed they can be differentiated again.  Eager calls only: tracing, ``torch.func`` and forward mode
+    are refused (``ShortConvolution`` goes through torch's conv1d there).
     """
     op = "causal_conv1d"
+    _rows.eager_only(op, x, weight, bias, initial_state)
     assert x.dim() == 3, f"{op}: expected x [B, T, D], got {tuple(x.shape)}"
     weight = _weight2d(op, weight)
     N, cu = _rows.sequences(op, cu_seqlens, x.shape[0], x.shape[1], x.device)
@@ -146,6 +148,7 @@ def causal_conv1d_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     given, which may be ``state`` itself (updated in place).  No gradient.
     """
     op = "causal_conv1d_step"
+    _rows.eager_only(op, x, state, weight, bias)
     assert x.dim() == 2, f"{op}: expected x [B, D], got {tuple(x.shape)}"
     weight = _weight2d(op, weight)
     B, D = x.shape

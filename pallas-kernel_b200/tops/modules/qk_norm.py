@@ -64,6 +64,7 @@ class _QKNormRotary(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dqo, dko):
+        _rows.eager_grads("qk_norm_rotary", dqo, dko)
         q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
         q, k = _rows.rows(q), _rows.rows(k)
         qw, kw = (None if w is None else w.contiguous() for w in (qw, kw))
@@ -135,9 +136,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
         positions: [T] or [B, T] int32 or int64; default 0..T-1.  A position outside 0..P-1 gives NaN in
             the rotated elements (the host does not read the positions).
         interleaved: the pairs are (2i, 2i + 1) instead of (i, i + R / 2)
-    Gradients flow to q, k and the weights.
+    Gradients flow to q, k and the weights.  Eager calls only: tracing, ``torch.func`` and forward mode are refused.
     """
     op = "qk_norm_rotary"
+    _rows.eager_only(op, q, k, q_weight, k_weight, cos, sin)
     assert q.dim() == 4 and k.dim() == 4, f"{op}: expected q [B, T, H, K] and k [B, T, HK, K]"
     B, T, _, K = q.shape
     if not 1 <= K <= MAX_HEAD:

@@ -71,6 +71,7 @@ class _SelectiveScan(torch.autograd.Function):
         need = ctx.needs_input_grad
         if dout is None and dht is None:
             return (None,) * 13
+        _rows.eager_grads("selective_scan", dout, dht)
         x, dt, A, Bm, Cm, D, z, bias, h0 = _dense(*inputs)
         new = lambda like: like.new_empty(like.shape)  # noqa: E731
         dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dout is None else _rows.rows(dout.to(x.dtype))
@@ -137,9 +138,11 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         cu_seqlens: [S + 1] offsets of S sequences packed along T (batch size 1).  Offsets on the GPU are
             not read by the host (capturable); rows behind the last sequence give zeros.
     x, dt, z, B and C may be slices of wider tensors (dense channels).  A, D, dt_bias and states are
-    used in fp32.  Gradients flow to every tensor, also from the final state.
+    used in fp32.  Gradients flow to every tensor, also from the final state.  Eager calls only: tracing,
+    ``torch.func`` and forward mode are refused.
     """
     op = "selective_scan"
+    _rows.eager_only(op, x, dt, A, B, C, D, z, dt_bias, initial_state)
     assert x.dim() == 3, f"{op}: expected x [B, T, D], got {tuple(x.shape)}"
     S, cu = _rows.sequences(op, cu_seqlens, x.shape[0], x.shape[1], x.device)
     B, C = _check(op, x.shape[:2], x, dt, A, B, C, D, z, dt_bias, initial_state, S)
@@ -163,6 +166,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     place).  No gradient.
     """
     op = "selective_scan_step"
+    _rows.eager_only(op, x, dt, A, B, C, state, D, z, dt_bias)
     assert x.dim() == 2, f"{op}: expected x [B, D], got {tuple(x.shape)}"
     Bsz, ch = x.shape
     B, C = _check(op, x.shape[:1], x, dt, A, B, C, D, z, dt_bias, state, Bsz)

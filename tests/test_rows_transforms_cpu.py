@@ -1,6 +1,7 @@
 """Which calls the row operators' kernels may take, decided without a device."""
 from __future__ import annotations
 
+import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
@@ -39,3 +40,28 @@ def test_short_convolution_of_fake_cuda_tensors():
         m = ShortConvolution(24, 4, bias=True)
         y, cache = m(torch.empty(2, 13, 24, device="cuda"), None, True)
     assert y.shape == (2, 13, 24) and cache.shape == (2, 24, 3) and y.device.type == "cuda"
+
+
+def test_operators_say_what_they_cannot_follow():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from tops.modules import causal_conv1d, causal_conv1d_step, qk_norm_rotary
+    from tops.ops.ssm import selective_scan, selective_scan_step
+    t = torch.randn
+    w, st, A, B, h, k = t(8, 4), t(2, 8, 3), t(8, 4), t(2, 4, 4), t(2, 8, 4), t(2, 4, 2, 8)
+    for name, f, x in (("causal_conv1d", lambda v: causal_conv1d(v, w)[0], t(2, 4, 8)),
+                       ("causal_conv1d_step", lambda v: causal_conv1d_step(v, st, w)[0], t(2, 8)),
+                       ("selective_scan", lambda v: selective_scan(v, v, A, B, B)[0], t(2, 4, 8)),
+                       ("selective_scan_step", lambda v: selective_scan_step(v, v, A, B[:, 0], B[:, 0], h)[0], t(2, 8)),
+                       ("qk_norm_rotary", lambda v: qk_norm_rotary(v, k)[0], t(2, 4, 2, 8))):
+        with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+            torch.jit.trace(f, x, check_trace=False)
+        with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+            make_fx(f)(x)
+        with pytest.raises(RuntimeError, match=f"{name} .*torch.func"):
+            torch.vmap(f)(x[None])
+        with torch._subclasses.FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            with pytest.raises(RuntimeError, match=f"{name} cannot run on fake"):
+                f(mode.from_tensor(x))
+        with fwAD.dual_level():
+            with pytest.raises(RuntimeError, match=f"{name} has no forward-mode"):
+                f(fwAD.make_dual(x, x))

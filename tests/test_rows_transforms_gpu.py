@@ -117,6 +117,60 @@ def test_short_convolution_sees_modes_and_compilers():
         _near("compiled", torch.compile(g, backend="eager")(x2.cuda())[0], c(x2.double())[0], SIZE)
 
 
+def _calls():
+    """Every operator as a function of one tensor that requires nothing, with its argument."""
+    from tops.modules import causal_conv1d, causal_conv1d_step, qk_norm_rotary
+    from tops.ops.ssm import selective_scan, selective_scan_step
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    w, st, A, B, C, h = r(16, 4), r(2, 16, 3), -torch.rand(16, 4, device="cuda"), r(2, 8, 4), r(2, 8, 4), r(2, 16, 4)
+    k = r(2, 8, 1, 16)
+    return {"causal_conv1d": (lambda x: causal_conv1d(x, w)[0], r(2, 8, 16)),
+            "causal_conv1d, weight": (lambda v: causal_conv1d(h.transpose(1, 2), v)[0], w),
+            "causal_conv1d_step": (lambda x: causal_conv1d_step(x, st, w)[0], r(2, 16)),
+            "selective_scan": (lambda x: selective_scan(x, x, A, B, C)[0], r(2, 8, 16)),
+            "selective_scan, C": (lambda c: selective_scan(h.new_ones(2, 8, 16), h.new_ones(2, 8, 16), A, B, c)[0], C),
+            "selective_scan_step": (lambda x: selective_scan_step(x, x, A, B[:, 0], C[:, 0], h)[0], r(2, 16)),
+            "qk_norm_rotary": (lambda q: qk_norm_rotary(q, k)[0], r(2, 8, 2, 16))}
+
+
+def test_operators_refuse_what_they_cannot_follow():
+    """No tangent is dropped, no empty tensor recorded, nothing run on tensors without memory."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for name, (f, x) in _calls().items():
+        op = name.split(",")[0]
+        f(x)
+        with torch.no_grad():
+            with pytest.raises(RuntimeError, match=f"{op}.*trac"):
+                torch.jit.trace(f, x, check_trace=False)
+            with fwAD.dual_level():
+                with pytest.raises(RuntimeError, match=f"{op}.*tangent"):
+                    f(fwAD.make_dual(x, torch.ones_like(x)))
+                f(x)  # a level without a tangent is nothing to refuse
+            with pytest.raises(RuntimeError, match=f"{op}.*trac"):
+                make_fx(f)(x)
+            with torch._subclasses.FakeTensorMode(allow_non_fake_inputs=True) as mode:
+                with pytest.raises(RuntimeError, match=f"{op}.*(fake|trac)"):
+                    f(mode.from_tensor(x))
+        for t in (lambda: torch.vmap(f)(x[None]), lambda: torch.func.jvp(f, (x,), (x,)),
+                  lambda: torch.func.grad(lambda v: f(v).sum())(x)):
+            with pytest.raises(RuntimeError, match=f"{op}.*torch.func"):
+                t()
+
+
+def test_backwards_refuse_what_they_cannot_follow():
+    for name, (f, x) in _calls().items():
+        if "step" in name or name.startswith("causal"):
+            continue
+        X = x.clone().requires_grad_()
+        y = f(X)
+        dy = torch.ones_like(y)
+        with fwAD.dual_level():
+            with pytest.raises(RuntimeError, match="tangent"):
+                torch.autograd.grad(y, X, fwAD.make_dual(dy, dy), retain_graph=True)
+        with pytest.raises(RuntimeError, match="torch.func"):
+            torch.autograd.grad(y, X, dy[None], is_grads_batched=True)
+
+
 def test_eager_short_convolution():
     """Eager calls stay on the kernel: its values within its own, tighter bound."""
     g, c = _pair(bias=False, D=40)
