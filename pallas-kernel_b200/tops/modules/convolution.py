@@ -65,7 +65,9 @@ class _CausalConv(torch.autograd.Function):
                 raise RuntimeError("causal_conv1d: packed sequences have no second derivative")
             leaves = [t for t, n in zip((x, w, bias, state), need) if n]
             y, final = _torch_form(x, w, bias, state, ctx.act)
-            pairs = [(o, g) for o, g in ((y, dy), (final, dfinal)) if g is not None]
+            pairs = [(o, g) for o, g in ((y, dy), (final, dfinal)) if g is not None and o.requires_grad]
+            if not pairs:  # the final state alone, of inputs that need no gradient
+                return (None,) * 8
             got = iter(torch.autograd.grad([o for o, _ in pairs], leaves, [g for _, g in pairs], create_graph=True,
                                            allow_unused=True))
             return tuple(next(got) if n else None for n in need[:4]) + (None,) * 4

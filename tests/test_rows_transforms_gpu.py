@@ -171,6 +171,43 @@ def test_backwards_refuse_what_they_cannot_follow():
             torch.autograd.grad(y, X, dy[None], is_grads_batched=True)
 
 
+# -- second derivatives of the convolution ----------------------------------------------------------------------
+
+
+def _second(dt, wdt, seed=5, B=2, T=11, D=8, W=4):
+    gen = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    return {"x": rn(B, T, D).to(dt), "w": (rn(D, W) / 2).to(wdt), "b": (rn(D) / 4).to(wdt), "st": rn(B, D, W - 1).to(dt),
+            "dy": rn(B, T, D).to(dt), "df": rn(B, D, W - 1).to(dt)}
+
+
+def _form(x, w, b, st):
+    T, W = x.shape[1], w.shape[1]
+    rows = torch.cat([st.transpose(1, 2), x], 1)
+    p = sum(rows[:, j:j + T] * w[:, j] for j in range(W)) + b
+    return torch.nn.functional.silu(p), rows[:, T:].transpose(1, 2)
+
+
+def test_create_graph_of_frozen_inputs():
+    """Only the weight is trained, and the final state, which does not depend on it, has a gradient too."""
+    from tops.modules import causal_conv1d
+    s = {k: v.cuda() for k, v in _second(torch.float32, torch.float32).items()}
+    w = s["w"].requires_grad_()
+    y, fin = causal_conv1d(s["x"], w, s["b"], "silu", s["st"], True)
+    (dw,) = torch.autograd.grad([y, fin], w, [s["dy"], s["df"]], create_graph=True)
+    (ddw,) = torch.autograd.grad(dw.square().sum(), w)
+    W2 = s["w"].detach().double().cpu().requires_grad_()
+    y2, _ = _form(s["x"].double().cpu(), W2, s["b"].double().cpu(), s["st"].double().cpu())
+    (want,) = torch.autograd.grad(y2, W2, s["dy"].double().cpu(), create_graph=True)
+    (ddwant,) = torch.autograd.grad(want.square().sum(), W2)
+    for a, b in ((dw, want), (ddw, ddwant)):
+        assert ((a.double().cpu() - b).norm() / b.norm()).item() <= 64 * 2 ** 6 * U32
+    # the final state alone
+    _, fin = causal_conv1d(s["x"], w, s["b"], "silu", s["st"], True)
+    (dw,) = torch.autograd.grad(fin, w, s["df"], create_graph=True, allow_unused=True)
+    assert dw is None or not dw.any()
+
+
 def test_eager_short_convolution():
     """Eager calls stay on the kernel: its values within its own, tighter bound."""
     g, c = _pair(bias=False, D=40)
