@@ -35,14 +35,75 @@ def _forward(x, w, bias, state, act, want_final, N, cu):
     return y, final
 
 
-def _torch_form(x, w, bias, state, act):
-    """The same in torch operations: what a second derivative is taken through."""
+def _backward(x, w, bias, state, dy, dfinal, act, N, cu, need):
+    """Gradients of x, w, bias and state from the kernel (None where not needed)."""
+    x = _rows.rows(x)
+    w, bias, state = (t if t is None else t.contiguous() for t in (w, bias, state))
+    dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _rows.rows(dy.to(x.dtype))
+    dfinal = None if dfinal is None else dfinal.to(x.dtype).contiguous()
+    dx = x.new_empty(x.shape)
+    dw = torch.empty_like(w) if need[1] else None
+    db = torch.empty_like(bias) if bias is not None and need[2] else None
+    ds = torch.empty_like(state) if state is not None and need[3] else None
+    a = _C.ConvBwdArgs(_args(x, w, bias, state, None, None, act, N, cu), dy.data_ptr(), dy.stride(0), dy.stride(1),
+                       _C.ptr(dfinal), dx.data_ptr(), _C.ptr(dw), _C.ptr(db), _C.ptr(ds), None, 0)
+    ws = _rows.workspace(_C.lib().tops_gla_causal_conv_bwd_workspace_size(a), x)
+    a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
+    _rows.launch("tops_gla_causal_conv_bwd", a, x)
+    return dx if need[0] else None, dw, db, ds
+
+
+def _gradient_form(x, w, bias, state, dy, dfinal, act, need):
+    """The same in elementary torch operations in 32 bits: what the gradients' own derivatives are taken through."""
     B, T, D = x.shape
     W = w.shape[1]
-    prev = x.new_zeros(B, D, W - 1) if state is None else state
-    xin = torch.cat([prev, x.transpose(1, 2)], -1)
-    y = F.conv1d(xin, w.to(x.dtype).unsqueeze(1), None if bias is None else bias.to(x.dtype), groups=D)
-    return (F.silu(y) if act else y).transpose(1, 2), xin[..., T:]
+    prev = x.new_zeros(B, W - 1, D) if state is None else state.transpose(1, 2)
+    rows, wf = torch.cat([prev, x], 1).float(), w.float()
+    d = x.new_zeros(B, T, D, dtype=torch.float32) if dy is None else dy.float()
+    if act:
+        p = sum(rows[:, j:j + T] * wf[:, j] for j in range(W)) + (0.0 if bias is None else bias.float())
+        s = torch.sigmoid(p)
+        d = d * s * (1 + p * (1 - s))
+    drows = dw = db = None
+    if need[0] or need[3]:
+        drows = sum(F.pad(d * wf[:, j], (0, 0, j, W - 1 - j)) for j in range(W))
+        if dfinal is not None:
+            drows = drows + F.pad(dfinal.float().transpose(1, 2), (0, 0, T, 0))
+    if need[1]:
+        dw = torch.stack([(d * rows[:, j:j + T]).sum((0, 1)) for j in range(W)], -1).to(w.dtype)
+    if bias is not None and need[2]:
+        db = d.sum((0, 1)).to(bias.dtype)
+    return (drows[:, W - 1:].to(x.dtype) if need[0] else None, dw, db,
+            drows[:, :W - 1].transpose(1, 2).to(x.dtype) if state is not None and need[3] else None)
+
+
+class _CausalConvGradient(torch.autograd.Function):
+    """The backward as an operation of its own (create_graph): the kernel's gradients, differentiated by their formula."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, state, dy, dfinal, act, N, cu, need):
+        ctx.save_for_backward(x, w, bias, state, dy, dfinal)
+        ctx.act, ctx.packed, ctx.need = act, cu is not None, need
+        ctx.set_materialize_grads(False)
+        return _backward(x, w, bias, state, dy, dfinal, act, N, cu, need)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        if ctx.packed:
+            raise RuntimeError("causal_conv1d: packed sequences have no second derivative")
+        again = torch.is_grad_enabled()
+        with torch.enable_grad():
+            # a view each: one tensor given in two places is two variables here
+            given = [None if t is None else t.view_as(t) for t in ctx.saved_tensors]
+            first = _gradient_form(*given, ctx.act, ctx.need)
+            pairs = [(f, g) for f, g in zip(first, grads) if g is not None and f.requires_grad]
+            wanted = [t for t, n in zip(given, ctx.needs_input_grad) if n]
+            if pairs and wanted:
+                got = iter(torch.autograd.grad([f for f, _ in pairs], wanted, [g for _, g in pairs], create_graph=again,
+                                               allow_unused=True))
+            else:
+                got = iter([None] * len(wanted))
+        return tuple(next(got) if n else None for n in ctx.needs_input_grad[:6]) + (None,) * 4
 
 
 class _CausalConv(torch.autograd.Function):
@@ -56,35 +117,13 @@ class _CausalConv(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dfinal=None):
-        x, w, bias, state, cu = ctx.saved_tensors
-        need = ctx.needs_input_grad
+        *inputs, cu = ctx.saved_tensors
+        need = ctx.needs_input_grad[:4]
         if dy is None and dfinal is None:
             return (None,) * 8
-        if torch.is_grad_enabled():  # create_graph: the gradient itself is differentiated
-            if cu is not None:
-                raise RuntimeError("causal_conv1d: packed sequences have no second derivative")
-            leaves = [t for t, n in zip((x, w, bias, state), need) if n]
-            y, final = _torch_form(x, w, bias, state, ctx.act)
-            pairs = [(o, g) for o, g in ((y, dy), (final, dfinal)) if g is not None and o.requires_grad]
-            if not pairs:  # the final state alone, of inputs that need no gradient
-                return (None,) * 8
-            got = iter(torch.autograd.grad([o for o, _ in pairs], leaves, [g for _, g in pairs], create_graph=True,
-                                           allow_unused=True))
-            return tuple(next(got) if n else None for n in need[:4]) + (None,) * 4
-        xr = _rows.rows(x)
-        w, bias, state = (t if t is None else t.contiguous() for t in (w, bias, state))
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _rows.rows(dy.to(x.dtype))
-        dfinal = None if dfinal is None else dfinal.to(x.dtype).contiguous()
-        dx = x.new_empty(x.shape)
-        dw = torch.empty_like(w) if need[1] else None
-        db = torch.empty_like(bias) if bias is not None and need[2] else None
-        ds = torch.empty_like(state) if state is not None and need[3] else None
-        a = _C.ConvBwdArgs(_args(xr, w, bias, state, None, None, ctx.act, ctx.N, cu), dy.data_ptr(), dy.stride(0),
-                           dy.stride(1), _C.ptr(dfinal), dx.data_ptr(), _C.ptr(dw), _C.ptr(db), _C.ptr(ds), None, 0)
-        ws = _rows.workspace(_C.lib().tops_gla_causal_conv_bwd_workspace_size(a), x)
-        a.workspace, a.workspace_bytes = _C.ptr(ws), 0 if ws is None else ws.numel()
-        _rows.launch("tops_gla_causal_conv_bwd", a, x)
-        return dx, dw, db, ds, None, None, None, None
+        a = (*inputs, dy, dfinal, ctx.act, ctx.N, cu, need)
+        got = _CausalConvGradient.apply(*a) if torch.is_grad_enabled() else _backward(*a)
+        return *got, None, None, None, None
 
 
 def _check(op, x, weight, bias, activation, D, state, state_shape):
@@ -126,7 +165,8 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
         cu_seqlens: [N + 1] offsets of N sequences packed along T (B must be 1).  Offsets on the GPU are
             not read by the host (capturable); rows behind the last sequence give zeros.
     Gradients flow to x, weight, bias and initial_state, also from the final state; where sequences
-    are not packed they can be differentiated again.  Eager calls only: tracing, ``torch.func`` and forward mode
+    are not packed they can be differentiated again (the first gradients stay the kernel's, the rest is taken in
+    fp32 torch operations).  Eager calls only: tracing, ``torch.func`` and forward mode
     are refused (``ShortConvolution`` goes through torch's conv1d there).
     """
     op = "causal_conv1d"

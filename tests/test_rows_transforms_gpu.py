@@ -188,6 +188,38 @@ def _form(x, w, b, st):
     return torch.nn.functional.silu(p), rows[:, T:].transpose(1, 2)
 
 
+@pytest.mark.parametrize("dt,wdt", [(torch.float32,) * 2, (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+def test_first_gradients_are_the_same_bits_with_create_graph(dt, wdt):
+    from tops.modules import causal_conv1d
+    s = {k: v.cuda().requires_grad_() for k, v in _second(dt, wdt).items()}
+    leaves = [s[k] for k in ("x", "w", "b", "st")]
+    got = []
+    for create in (False, True):
+        y, fin = causal_conv1d(s["x"], s["w"], s["b"], "silu", s["st"], True)
+        got.append(torch.autograd.grad([y, fin], leaves, [s["dy"], s["df"]], create_graph=create))
+    assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(*got))
+    assert all(g.requires_grad for g in got[1])
+
+
+def test_second_and_third_derivatives_in_full_precision():
+    from tops.modules import causal_conv1d
+    cpu = _second(torch.float32, torch.float32)
+    names = ("x", "w", "b", "st", "dy", "df")
+    res = []
+    for f, s in ((lambda *a: causal_conv1d(a[0], a[1], a[2], "silu", a[3], True), {k: v.cuda() for k, v in cpu.items()}),
+                 (_form, {k: v.double() for k, v in cpu.items()})):
+        s = {k: v.requires_grad_() for k, v in s.items()}
+        y, fin = f(*(s[k] for k in names[:4]))
+        first = torch.autograd.grad([y, fin], [s[k] for k in names[:4]], [s["dy"], s["df"]], create_graph=True)
+        second = torch.autograd.grad(sum(g.square().sum() for g in first), [s[k] for k in names], create_graph=True)
+        third = torch.autograd.grad(sum(g.square().sum() for g in second), [s[k] for k in names[:4]])
+        res.append((*first, *second, *third))
+    # each derivative adds at most 64 roundings to terms whose sums do not cancel by more than 2^6 here
+    for i, (a, b) in enumerate(zip(*res)):
+        rel = ((a.double().cpu() - b).norm() / b.norm()).item()
+        assert rel <= 64 * 2 ** 6 * U32, f"{i}: {rel:.2e}"
+
+
 def test_create_graph_of_frozen_inputs():
     """Only the weight is trained, and the final state, which does not depend on it, has a gradient too."""
     from tops.modules import causal_conv1d
@@ -206,6 +238,37 @@ def test_create_graph_of_frozen_inputs():
     _, fin = causal_conv1d(s["x"], w, s["b"], "silu", s["st"], True)
     (dw,) = torch.autograd.grad(fin, w, s["df"], create_graph=True, allow_unused=True)
     assert dw is None or not dw.any()
+
+
+def test_create_graph_of_packed_rows():
+    """First gradients as without it; the second is refused."""
+    from tops.modules import causal_conv1d
+    s = {k: v.cuda() for k, v in _second(torch.float32, torch.float32).items()}
+    w = s["w"].requires_grad_()
+    X = s["x"].reshape(1, 22, 8).requires_grad_()
+    args = (X, w, s["b"], "silu", s["st"], False, [0, 11, 22])
+    y, _ = causal_conv1d(*args)
+    dy = s["dy"].reshape(1, 22, 8)
+    (dx,) = torch.autograd.grad(y, X, dy, create_graph=True)
+    (dx2,) = torch.autograd.grad(causal_conv1d(*args)[0], X, dy)
+    assert torch.equal(dx, dx2)
+    with pytest.raises(RuntimeError, match="packed sequences"):
+        torch.autograd.grad(dx.sum(), X)
+
+
+def test_one_tensor_in_two_places():
+    """The gradient that goes in is the input itself: both ways count once."""
+    from tops.modules import causal_conv1d
+    s = {k: v.cuda() for k, v in _second(torch.float32, torch.float32).items()}
+    X = s["x"].requires_grad_()
+    y, _ = causal_conv1d(X, s["w"], s["b"], "silu", s["st"])
+    (dx,) = torch.autograd.grad(y, X, X, create_graph=True)
+    (got,) = torch.autograd.grad(dx.square().sum(), X)
+    X2 = s["x"].detach().double().cpu().requires_grad_()
+    y2, _ = _form(X2, *(s[k].double().cpu() for k in ("w", "b", "st")))
+    (dx2,) = torch.autograd.grad(y2, X2, X2, create_graph=True)
+    (want,) = torch.autograd.grad(dx2.square().sum(), X2)
+    assert ((got.double().cpu() - want).norm() / want.norm()).item() <= 64 * 2 ** 6 * U32
 
 
 def test_eager_short_convolution():
