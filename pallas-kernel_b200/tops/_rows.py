@@ -39,8 +39,13 @@ def eager_only(op: str, *tensors) -> None:
         raise RuntimeError(f"{op} has no forward-mode derivative: a tensor carries a tangent")
 
 
+def plain_grads(*grads) -> bool:
+    """``plain`` for the gradients that a backward is given (it may run on another thread than a transform)."""
+    return plain(*grads) and all(g is None or _has_storage(g) for g in grads)
+
+
 def eager_grads(op: str, *grads) -> None:
-    """``eager_only`` for the gradients that a backward is given (it may run on another thread than a transform)."""
+    """``eager_only`` for the gradients that a backward is given."""
     eager_only(op, *grads)
     for g in grads:
         if g is not None and not _has_storage(g):

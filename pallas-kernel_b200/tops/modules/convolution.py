@@ -121,6 +121,10 @@ class _CausalConv(torch.autograd.Function):
         need = ctx.needs_input_grad[:4]
         if dy is None and dfinal is None:
             return (None,) * 8
+        if not _rows.plain_grads(dy, dfinal):  # a batch of gradients, a tangent, a mode: the formula carries them
+            if cu is None:
+                return *_gradient_form(*inputs, dy, dfinal, ctx.act, need), None, None, None, None
+            _rows.eager_grads("causal_conv1d of packed sequences", dy, dfinal)
         a = (*inputs, dy, dfinal, ctx.act, ctx.N, cu, need)
         got = _CausalConvGradient.apply(*a) if torch.is_grad_enabled() else _backward(*a)
         return *got, None, None, None, None

@@ -100,6 +100,49 @@ def test_short_convolution_under_torch_func():
         _near(k, got[k], want[k], 20 * SIZE, 256)  # gradients of a square: one product more, sums of 18 rows
 
 
+def test_batched_gradients_of_short_convolution():
+    g, c = _pair()
+    x, dy = torch.randn(2, 7, 24), torch.randn(3, 2, 7, 24)
+    got, want = [], []
+    for m, cast, out in ((g, lambda v: v.cuda(), got), (c, lambda v: v.double(), want)):
+        X = cast(x).requires_grad_()
+        y, _ = m(X)
+        out.extend(torch.autograd.grad(y, [X, *m.parameters()], cast(dy), is_grads_batched=True))
+    for i, (a, b) in enumerate(zip(got, want)):
+        _near(str(i), a, b, SIZE, 256)
+
+
+def test_tangent_of_the_gradient_reaches_the_input():
+    """The gradient that goes in carries a tangent; dx is linear in it, so its tangent is the tangent's own gradient."""
+    g, c = _pair()
+    x, dy, t = (torch.randn(2, 7, 24) for _ in range(3))
+    X, Xc = x.cuda().requires_grad_(), x.double().requires_grad_()
+    y, _ = g(X)
+    with fwAD.dual_level():
+        (dx,) = torch.autograd.grad(y, X, fwAD.make_dual(dy.cuda(), t.cuda()))
+        value, tangent = fwAD.unpack_dual(dx)
+    assert tangent is not None
+    yc, _ = c(Xc)
+    for name, got, d in (("dx", value, dy), ("tangent", tangent, t)):
+        _near(name, got, torch.autograd.grad(yc, Xc, d.double(), retain_graph=True)[0], SIZE)
+
+
+def test_packed_gradients_refuse_batches_and_tangents():
+    from tops.modules import causal_conv1d
+    X, w = torch.randn(1, 12, 8, device="cuda").requires_grad_(), torch.randn(8, 4, device="cuda")
+    y, _ = causal_conv1d(X, w, cu_seqlens=[0, 5, 12])
+    dy = torch.randn(1, 12, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="batch"):
+        torch.autograd.grad(y, X, dy[None], is_grads_batched=True)
+    with fwAD.dual_level():
+        with pytest.raises(RuntimeError, match="tangent"):
+            torch.autograd.grad(y, X, fwAD.make_dual(dy, dy), retain_graph=True)
+    from torch.utils.flop_counter import FlopCounterMode
+    with FlopCounterMode(display=False):  # a mode that only looks on
+        (a,) = torch.autograd.grad(y, X, dy, retain_graph=True)
+    assert torch.equal(a, torch.autograd.grad(y, X, dy)[0])
+
+
 def test_short_convolution_sees_modes_and_compilers():
     from torch.fx.experimental.proxy_tensor import make_fx
     from torch.utils.flop_counter import FlopCounterMode
