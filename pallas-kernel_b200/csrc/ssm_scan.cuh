@@ -327,7 +327,7 @@ inline void split(P& p, int blocks_per_row, int wanted, int resident) {
   p.seg = std::max(p.T, 1);
   p.nseg = 1;
   const int64_t blocks = (int64_t)blocks_per_row * p.B, slots = kSms * resident;
-  if (blocks >= wanted || p.T < 2 * kMinSegment) return;
+  if (blocks == 0 || blocks >= wanted || p.T < 2 * kMinSegment) return;
   int64_t best = INT64_MAX;
   for (int waves = 2; waves <= 4; ++waves) {
     const int want = (int)std::min<int64_t>(waves * slots / blocks, p.T / kMinSegment);

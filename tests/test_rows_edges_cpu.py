@@ -1,0 +1,34 @@
+"""The row operators' C entry points at sizes of zero and past their types, without a device."""
+from __future__ import annotations
+
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+PKG = Path(__file__).resolve().parents[1] / "pallas-kernel_b200"
+
+
+@pytest.fixture(scope="module")
+def C():
+    import build as B  # pallas-kernel_b200/build.py (incremental)
+    B.build()
+    from tops import _C
+    return _C
+
+
+def test_scan_of_no_batch_rows_has_a_plan(C):
+    """Long rows, none of them: the plan divided by the number of blocks (in a process of its own, which that ended)."""
+    code = """
+import ctypes
+from tops import _C as C
+a = C.ScanArgs(B=0, T=4096, D=8, N=16, G=1, S=0, dtype=C.BF16)
+b = C.ScanBwdArgs(f=a)
+L = C.lib()
+print(L.tops_gla_ssm_scan_states_size(ctypes.byref(a)), L.tops_gla_ssm_scan_fwd_workspace_size(ctypes.byref(a)),
+      L.tops_gla_ssm_scan_bwd_workspace_size(ctypes.byref(b)))
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=PKG, capture_output=True, text=True)
+    assert r.returncode == 0, f"exit {r.returncode}: {r.stderr[-300:]}"
+    assert r.stdout.split() == ["0", "0", "0"]
