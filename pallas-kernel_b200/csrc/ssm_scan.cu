@@ -361,6 +361,7 @@ TOPS_API int tops_gla_ssm_scan_fwd(const tops_gla_scan_args* a, void* stream) {
   if (int rc = check(a)) return rc;
   const bool rows = (int64_t)a->B * a->T > 0;
   TOPS_CHECK_ARG(!rows || (a->x && a->dt && a->Bm && a->Cm && a->A && a->y), "ssm_scan_fwd: x, dt, B, C, A and y are required");
+  TOPS_CHECK_ARG(rows || a->B == 0 || !a->ht || a->A, "ssm_scan_fwd: the final state needs A");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   P p = params(a);
   const size_t need = plan_fwd(p, a->workspace);

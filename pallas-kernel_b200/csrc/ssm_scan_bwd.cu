@@ -591,6 +591,7 @@ TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream
   const bool rows = (int64_t)f.B * f.T > 0;
   TOPS_CHECK_ARG(!rows || (f.x && f.dt && f.Bm && f.Cm && f.A && f.states && a->dout && a->dx && a->ddt && a->dB && a->dC),
                  "ssm_scan_bwd: x, dt, B, C, A, states, dout and the gradients of x, dt, B and C are required");
+  TOPS_CHECK_ARG(f.B == 0 || f.A, "ssm_scan_bwd: A is required");
   TOPS_CHECK_ARG(!rows || !f.z || a->dz, "ssm_scan_bwd: z needs dz");
   TOPS_CHECK_ARG(aligned_to(a->workspace, 16), "ssm_scan_bwd: workspace must be 16-byte aligned");
   P p = params(&f);

@@ -1,6 +1,7 @@
 """The row operators' C entry points at sizes of zero and past their types, without a device."""
 from __future__ import annotations
 
+import ctypes
 import subprocess
 import sys
 from pathlib import Path
@@ -32,3 +33,17 @@ print(L.tops_gla_ssm_scan_states_size(ctypes.byref(a)), L.tops_gla_ssm_scan_fwd_
     r = subprocess.run([sys.executable, "-c", code], cwd=PKG, capture_output=True, text=True)
     assert r.returncode == 0, f"exit {r.returncode}: {r.stderr[-300:]}"
     assert r.stdout.split() == ["0", "0", "0"]
+
+
+def test_scan_without_rows_needs_its_matrix(C):
+    """Without rows the kernels still carry states from h0 to ht and read A for it."""
+    a = C.ScanArgs(B=1, T=0, D=8, N=16, G=1, S=1, dtype=C.BF16, ht=16)
+    assert C.lib().tops_gla_ssm_scan_fwd(ctypes.byref(a), None) == -1
+    assert "A" in C.lib().tops_gla_last_error().decode()
+    a.ht = None  # nothing to do
+    assert C.lib().tops_gla_ssm_scan_fwd(ctypes.byref(a), None) == 0
+    n = C.lib().tops_gla_ssm_scan_bwd_workspace_size(ctypes.byref(C.ScanBwdArgs(f=a)))
+    assert n > 0
+    b = C.ScanBwdArgs(f=a, workspace=256, workspace_bytes=n)
+    assert C.lib().tops_gla_ssm_scan_bwd(ctypes.byref(b), None) == -1
+    assert "A" in C.lib().tops_gla_last_error().decode()
