@@ -467,8 +467,8 @@ TOPS_API int tops_gla_causal_conv_step(const tops_gla_conv_args* a, void* stream
  * x, dt, z [B,T,D] and Bm, Cm [B,T,G,N] in dtype, strides in elements (batch, row; the rest
  * contiguous); A [D,N], skip [D], dt_bias [D], h0 / ht [S,D,N] fp32; skip, dt_bias, z, h0, ht may be
  * NULL; N in 1..64; G divides D.  cu_seqlens as in the convolution (S sequences; S == B without).
- * `states` (tops_gla_ssm_scan_states_size() bytes, or NULL) keeps what the backward starts from.  ht,
- * states and workspace are 16-byte aligned. */
+ * `states` (tops_gla_ssm_scan_states_size() bytes, or NULL) keeps what the backward starts from.  workspace
+ * is 16-byte aligned, and so are the forward's ht and states where N is a multiple of 4 above 8. */
 typedef struct tops_gla_scan_args {
   int32_t B, T, D, N, G, S, dtype, softplus;
   const int32_t* cu_seqlens;

@@ -361,6 +361,8 @@ TOPS_API int tops_gla_ssm_scan_fwd(const tops_gla_scan_args* a, void* stream) {
   if (int rc = check(a)) return rc;
   const bool rows = (int64_t)a->B * a->T > 0;
   TOPS_CHECK_ARG(!rows || (a->x && a->dt && a->Bm && a->Cm && a->A && a->y), "ssm_scan_fwd: x, dt, B, C, A and y are required");
+  TOPS_CHECK_ARG(a->N <= 8 || a->N % 4 || (aligned_to(a->ht, 16) && aligned_to(a->states, 16)),
+                 "ssm_scan_fwd: ht and states must be 16-byte aligned (their four states a thread are one store)");
   TOPS_CHECK_ARG(rows || a->B == 0 || !a->ht || a->A, "ssm_scan_fwd: the final state needs A");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   P p = params(a);

@@ -47,3 +47,15 @@ def test_scan_without_rows_needs_its_matrix(C):
     b = C.ScanBwdArgs(f=a, workspace=256, workspace_bytes=n)
     assert C.lib().tops_gla_ssm_scan_bwd(ctypes.byref(b), None) == -1
     assert "A" in C.lib().tops_gla_last_error().decode()
+
+
+def test_scan_states_at_any_place(C):
+    """Only the forward stores four states at once, and only where N is a multiple of 4 above 8."""
+    at = lambda T, N, ht, **kw: C.ScanArgs(B=1, T=T, D=8, N=N, G=1, S=1, dtype=C.BF16, ht=ht, **kw)  # noqa: E731
+    L = C.lib()
+    for N, ht, ok in ((16, 24, False), (16, 32, True), (8, 24, True), (11, 4, True), (12, 8, False)):
+        # the arguments are looked at in order: an unaligned state is refused before what is missing
+        assert L.tops_gla_ssm_scan_fwd(ctypes.byref(at(0, N, ht)), None) == -1
+        assert ("aligned" not in L.tops_gla_last_error().decode()) == ok
+        assert L.tops_gla_ssm_scan_step(ctypes.byref(at(1, N, ht)), None) == -1
+        assert "required" in L.tops_gla_last_error().decode()
