@@ -369,7 +369,7 @@ TOPS_API int tops_gla_ssm_scan_fwd(const tops_gla_scan_args* a, void* stream) {
   const size_t need = plan_fwd(p, a->workspace);
   if (need && (a->workspace == nullptr || a->workspace_bytes < need))
     return fail(TOPS_ERR_WORKSPACE, "ssm_scan_fwd: workspace smaller than tops_gla_ssm_scan_fwd_workspace_size()");
-  if (int rc = empty_states(p, p.h0, p.ht, st)) return rc;
+  if (int rc = empty_states(p, p.h0, p.ht, false, st)) return rc;
   if (p.B == 0 || (!rows && !p.ht)) return TOPS_OK;
   if (p.nseg > 1) {
     LaunchTimer lt(st, "ssm_scan_sum");

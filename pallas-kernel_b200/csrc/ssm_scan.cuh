@@ -232,12 +232,12 @@ __global__ void __launch_bounds__(128) k_scan_chain(const P p) {
   }
 }
 
-// Packed sequences without rows: their final state is their initial one (and its gradient the
-// final state's).
+// Packed sequences without rows: their final state is their initial one (and its gradient the final state's).  So is
+// that of a sequence whose last (first) row falling offsets give to another one: nobody else would write it.
 static __global__ void k_scan_empty(int S, int T, int64_t DN, const int32_t* __restrict__ cu, const float* __restrict__ from,
-                             float* __restrict__ to) {
-  const int n = blockIdx.y;
-  if (min(cu[n + 1], T) > max(cu[n], 0)) return;
+                                    float* __restrict__ to, bool back) {
+  const int n = blockIdx.y, s = max(cu[n], 0), e = min(cu[n + 1], T);
+  if (e > s && seq_at(cu, S, T, back ? s : e - 1).n == n) return;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < DN; i += (int64_t)gridDim.x * blockDim.x)
     to[n * DN + i] = from ? from[n * DN + i] : 0.f;
 }
@@ -359,11 +359,11 @@ int by_type(int dtype, F f) {
   return f(__half());
 }
 
-inline int empty_states(const P& p, const float* from, float* to, cudaStream_t st) {
+inline int empty_states(const P& p, const float* from, float* to, bool back, cudaStream_t st) {
   if (!p.cu || !to) return TOPS_OK;
   LaunchTimer lt(st, "ssm_scan_empty");
   const int64_t dn = (int64_t)p.D * p.N;
-  k_scan_empty<<<dim3((unsigned)std::min<int64_t>((dn + 255) / 256, 64), p.S), 256, 0, st>>>(p.S, p.T, dn, p.cu, from, to);
+  k_scan_empty<<<dim3((unsigned)std::min<int64_t>((dn + 255) / 256, 64), p.S), 256, 0, st>>>(p.S, p.T, dn, p.cu, from, to, back);
   TOPS_CUDA_LAUNCH_CHECK("ssm_scan_empty");
   return TOPS_OK;
 }

@@ -601,7 +601,7 @@ TOPS_API int tops_gla_ssm_scan_bwd(const tops_gla_scan_bwd_args* a, void* stream
   p.dout = a->dout; p.os[0] = a->dout_stride_b; p.os[1] = a->dout_stride_t;
   p.dht = a->dht; p.dx = a->dx; p.ddt = a->ddt; p.dz = a->dz; p.dh0 = a->dh0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = empty_states(p, p.dht, p.dh0, st)) return rc;
+  if (int rc = empty_states(p, p.dht, p.dh0, true, st)) return rc;
   if (p.B > 0) {
     const int es = dtype_bytes(f.dtype);
     const bool ch4 = p.D / p.G % 4 == 0;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from _rows_ref import close, scan_ref
-from test_ssm_scan_gpu import NAMES, _dbl, _mk, _roundings
+from test_ssm_scan_gpu import NAMES, _call, _dbl, _mk, _roundings
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,44 @@ def test_scan_step_in_place_on_a_slice_of_a_cache(ch, N, off):
     close("state", s, *r["ht"], n)
     rest = torch.cat([cache[:off], cache[off + 2 * ch * N:]])
     assert torch.equal(rest, torch.full_like(rest, 7.0))
+
+
+def _used_memory(*shapes):
+    """Leaves NaN in the blocks that the next tensors of these shapes are given."""
+    held = [torch.full(s, float("nan"), device="cuda") for s in shapes for _ in range(4)]
+    del held
+
+
+@pytest.mark.parametrize("cu,lost,lost_back", [([0, 30, 12, 40], [1], [1, 2]), ([0, 40, 12, 20], [1, 2], [1, 2]),
+                                               ([25, 3, 40, 40], [0, 2], [0, 2])])
+def test_scan_falling_offsets_leave_nothing_unwritten(cu, lost, lost_back):
+    """Wrong rows, but every state and gradient is written: a sequence whose last (first) row another one has keeps its
+    initial state (the gradient of its final one)."""
+    T, S, ch, N = 40, 3, 64, 16
+    t, dout, dht = _mk(32, 1, T, ch, N, 1, torch.float32, S)
+    c = {k: v.cuda().requires_grad_() for k, v in t.items()}
+    off = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    _used_memory((S, ch, N))
+    y, ht = _call(c, True, off)
+    dht = dht.cuda()
+    _used_memory((S, ch, N))
+    g = dict(zip(NAMES, torch.autograd.grad([y, ht], [c[k] for k in NAMES], [dout.cuda(), dht])))
+    assert all(torch.isfinite(v).all() for v in (y, ht, *g.values()))
+    for n in lost:
+        assert torch.equal(ht[n], c["h0"][n])
+    for n in lost_back:
+        assert torch.equal(g["h0"][n], dht[n])
+
+
+@pytest.mark.parametrize("cu", [[0, 30, 12, 40], [0, 40, 12, 20], [25, 3, 40, 40]])
+@pytest.mark.parametrize("D", [64, 37])
+def test_conv_falling_offsets_leave_nothing_unwritten(cu, D):
+    from tops.modules import causal_conv1d
+    r = lambda *s: torch.randn(*s, device="cuda").requires_grad_()  # noqa: E731
+    x, w, b, st = r(1, 40, D), r(D, 4), r(D), r(3, D, 3)
+    off = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    _used_memory((1, 40, D), (3, D, 3), (D, 4))
+    y, fin = causal_conv1d(x, w, b, "silu", st, True, off)
+    _used_memory((1, 40, D), (3, D, 3), (D, 4))
+    g = torch.autograd.grad([y, fin], [x, w, b, st], [torch.ones_like(y), torch.ones_like(fin)])
+    assert all(torch.isfinite(v).all() for v in (y, fin, *g))
