@@ -200,6 +200,14 @@ __device__ __forceinline__ int row_flags(const P& p, int t, int& n) {
   return q.n < 0 ? kNone : (t == q.s ? kFirst : 0) | (t == q.e - 1 ? kLast : 0);
 }
 
+// own + 2^e c.  Decays grow where A and delta have one sign; over a segment 2^e alone may pass fp32 there: a state of
+// zero stays zero, and a small one is multiplied by the root twice.
+__device__ __forceinline__ float carried(float e, float c, float own) {
+  if (e <= 126.f) return fmaf(ex2(e), c, own);
+  const float root = ex2(0.5f * e);
+  return c == 0.f ? own : fmaf(root, root * c, own);
+}
+
 // Chains the segments: slot k becomes what segment k starts from.  Forward: slot 0 is not read by the main pass
 // (segment 0's own pass began with h0).  Backward: from the last segment, which starts from dht (packed: zero).
 template <bool BACK>
@@ -212,14 +220,14 @@ __global__ void __launch_bounds__(128) k_scan_chain(const P p) {
   float c = BACK && p.dht && !p.cu ? p.dht[b * dn + i] : 0.f;
   constexpr int U = 8;  // segments whose loads are in flight together
   for (int s0 = 0; s0 < p.nseg; s0 += U) {
-    float own[U], decay[U];
+    float own[U], e[U];
     bool cut[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u, k = BACK ? p.nseg - 1 - s : s;
       if (s >= p.nseg - 1) continue;  // the last segment passes nothing on
       own[u] = p.carry[((int64_t)b * p.nseg + k) * dn + i];
-      decay[u] = ex2(A * p.sdelta[((int64_t)b * p.nseg + k) * p.D + ch]);
+      e[u] = A * p.sdelta[((int64_t)b * p.nseg + k) * p.D + ch];
       cut[u] = (p.cu && p.broken[k]) || (!BACK && s == 0);  // segment 0 forward began with h0 itself
     }
 #pragma unroll
@@ -227,7 +235,7 @@ __global__ void __launch_bounds__(128) k_scan_chain(const P p) {
       const int s = s0 + u, k = BACK ? p.nseg - 1 - s : s;
       if (s >= p.nseg) break;
       p.carry[((int64_t)b * p.nseg + k) * dn + i] = c;
-      if (s < p.nseg - 1) c = cut[u] ? own[u] : fmaf(decay[u], c, own[u]);
+      if (s < p.nseg - 1) c = cut[u] ? own[u] : carried(e[u], c, own[u]);
     }
   }
 }

@@ -94,3 +94,47 @@ def test_conv_falling_offsets_leave_nothing_unwritten(cu, D):
     _used_memory((1, 40, D), (3, D, 3), (D, 4))
     g = torch.autograd.grad([y, fin], [x, w, b, st], [torch.ones_like(y), torch.ones_like(fin)])
     assert all(torch.isfinite(v).all() for v in (y, fin, *g))
+
+
+def _growing(T, ch, N):
+    """A > 0: the state grows by exp(A dt) a row; all inputs zero."""
+    t, _, _ = _mk(33, 1, T, ch, N, 1, torch.float32, 1, z=False, skip=False, bias=False)
+    t["A"], t["dt"] = torch.full((ch, N), 0.7), torch.full((1, T, ch), 0.01)
+    t["x"], t["h0"] = torch.zeros(1, T, ch), torch.zeros(1, ch, N)
+    return t
+
+
+def test_scan_growth_of_nothing_over_long_segments():
+    """Rows in which the decay's product passes fp32 while the state (the gradient) is zero: as row by row."""
+    T, ch, N = 512, 8, 4
+    g = torch.Generator().manual_seed(33)
+    t = _growing(T, ch, N)
+    t["dt"][:, :400] = 4.0  # exp(2.8) a row
+    t["x"][:, 400:] = torch.randn(1, 112, ch, generator=g)
+    y, ht = _call({k: None if v is None else v.cuda() for k, v in t.items()}, False, None)
+    r = scan_ref(*(_dbl(t[k]) for k in NAMES), False, None)
+    close("out", y, *r["out"], _roundings(112, N, ch, T))
+    close("ht", ht, *r["ht"], _roundings(112, N, ch, T))
+    t = _growing(T, ch, N)
+    t["dt"][:, 100:] = 4.0
+    dout = torch.zeros(1, T, ch)
+    dout[:, :100] = torch.randn(1, 100, ch, generator=g)
+    c = {k: None if v is None else v.cuda().requires_grad_() for k, v in t.items()}
+    y, _ = _call(c, False, None)
+    got = torch.autograd.grad(y, [c[k] for k in ("x", "dt", "A", "B", "C", "h0")], dout.cuda())
+    r = scan_ref(*(_dbl(t[k]) for k in NAMES), False, None, _dbl(dout), None)
+    for k, v in zip(("x", "dt", "A", "B", "C", "h0"), got):
+        close("d" + k, v, *r["d" + k], _roundings(100, N, ch, T))
+
+
+def test_scan_growth_of_a_small_state():
+    """exp(100) over one segment, from 1e-30: the product is in range though its factor is not."""
+    T, ch, N = 512, 8, 4
+    t = _growing(T, ch, N)
+    t["h0"] += 1e-30
+    t["dt"][:, :] = 1e-3
+    t["dt"][:, 64:128] = 100 / 64 / 0.7
+    _, ht = _call({k: None if v is None else v.cuda() for k, v in t.items()}, False, None)
+    want = scan_ref(*(_dbl(t[k]) for k in NAMES), False, None)["ht"][0]
+    # the exponent, about 100, is a sum of 64 rounded terms, and four roundings more
+    assert ((ht.double().cpu() - want).abs() <= 100 * 68 * 2.0 ** -24 * want).all()
