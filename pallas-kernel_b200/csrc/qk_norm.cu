@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kThreads) k_qk_bwd(const P p) {
       ex = group_sum(ex, p.lanes);
       if (!on) continue;
       const float s = rsqrtf(fmaf(ss, p.inv_k, p.eps));
-      const float m = s * s * s * ex * p.inv_k;
+      const float m = s * (s * (s * ex)) * p.inv_k;  // in this order every product is in range: x s is of order 1
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int e0 = (l + j * p.lanes) * V;

@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from _rows_ref import close, scan_ref
+from _rows_ref import close, qk_ref, scan_ref
 from test_ssm_scan_gpu import NAMES, _call, _dbl, _mk, _roundings
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +138,18 @@ def test_scan_growth_of_a_small_state():
     want = scan_ref(*(_dbl(t[k]) for k in NAMES), False, None)["ht"][0]
     # the exponent, about 100, is a sum of 64 rounded terms, and four roundings more
     assert ((ht.double().cpu() - want).abs() <= 100 * 68 * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.parametrize("scale,eps", [(1e-14, 0.0), (1e-14, 1e-30), (1e14, 1e-6), (1e-3, 1e-6)])
+@pytest.mark.parametrize("K", [64, 33])
+def test_qk_norm_backward_of_far_scales(scale, eps, K):
+    """1 / rms to the third power is out of fp32's range there, dx is not."""
+    from tops.modules import qk_norm_rotary
+    g = torch.Generator().manual_seed(34)
+    q, dq = torch.randn(1, 7, 2, K, generator=g) * scale, torch.randn(1, 7, 2, K, generator=g)
+    Q = q.cuda().requires_grad_()
+    y, _ = qk_norm_rotary(Q, q[:, :, :1].cuda(), eps=eps)
+    (dx,) = torch.autograd.grad(y, Q, dq.cuda())
+    ref = qk_ref(q.double(), None, None, None, None, eps, False, dq.double())
+    close("y", y, ref[0], ref[1], 2 * K + 24)
+    close("dx", dx, ref[2], ref[3], 2 * K + 24)
