@@ -6,6 +6,7 @@ import torch
 from torch._C import _get_dispatch_mode, _has_storage, _is_tracing, _len_torch_dispatch_stack, _TorchDispatchModeKey
 from torch._C._functorch import peek_interpreter_stack
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _C
 
@@ -126,7 +127,8 @@ def sequences(op: str, cu_seqlens, B: int, T: int, device) -> tuple[int, torch.T
 
 def state_target(op: str, state: torch.Tensor, out: torch.Tensor | None, *reads) -> tuple:
     """(state to read, tensor to write): ``out`` may be ``state`` itself; any other overlap with
-    what the call reads is refused."""
+    what the call reads is refused.  ``out`` counts as changed in place, so that a backward which still
+    needs what it held says so."""
     if out is None:
         state = state.contiguous()
         return state, torch.empty_like(state)
@@ -134,6 +136,8 @@ def state_target(op: str, state: torch.Tensor, out: torch.Tensor | None, *reads)
     if out.device != state.device:
         raise RuntimeError(f"{op}: state_out is on {out.device}, expected {state.device}")
     assert out.is_contiguous(), f"{op}: state_out must be contiguous"
+    if wants_grad(out):
+        raise RuntimeError(f"{op}: state_out requires a gradient, which the step does not have")
     a, n = out.data_ptr(), out.numel() * out.element_size()
     same = state.data_ptr() == a and state.is_contiguous()
     for t in reads if same else (state, *reads):
@@ -141,7 +145,9 @@ def state_target(op: str, state: torch.Tensor, out: torch.Tensor | None, *reads)
             last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
             if t.data_ptr() < a + n and a < t.data_ptr() + (last + 1) * t.element_size():
                 raise ValueError(f"{op}: state_out overlaps a tensor that the call reads")
-    return (state if same else state.contiguous()), out
+    state = state if same else state.contiguous()
+    increment_version(out)
+    return state, out
 
 
 def launch(name: str, args, t: torch.Tensor) -> None:

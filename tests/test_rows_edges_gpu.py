@@ -153,3 +153,22 @@ def test_qk_norm_backward_of_far_scales(scale, eps, K):
     ref = qk_ref(q.double(), None, None, None, None, eps, False, dq.double())
     close("y", y, ref[0], ref[1], 2 * K + 24)
     close("dx", dx, ref[2], ref[3], 2 * K + 24)
+
+
+def test_a_step_in_place_is_seen_by_the_backward():
+    """A prompt's state that a gradient still needs, then a step into it: the backward says so."""
+    from tops.modules import causal_conv1d, causal_conv1d_step
+    from tops.ops.ssm import selective_scan, selective_scan_step
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    x, w, st = r(2, 9, 16).requires_grad_(), r(16, 4), r(2, 16, 3)
+    y, _ = causal_conv1d(x, w, None, None, st)
+    with torch.no_grad():
+        causal_conv1d_step(x[:, 0], st, w, state_out=st)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    A, B, h = -torch.rand(16, 4, device="cuda"), r(2, 9, 4), r(2, 16, 4)
+    y, _ = selective_scan(x, x, A, B, B, initial_state=h)
+    with torch.no_grad():
+        selective_scan_step(x[:, 0], x[:, 0], A, B[:, 0], B[:, 0], h, state_out=h)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()

@@ -65,3 +65,21 @@ def test_operators_say_what_they_cannot_follow():
         with fwAD.dual_level():
             with pytest.raises(RuntimeError, match=f"{name} has no forward-mode"):
                 f(fwAD.make_dual(x, x))
+
+
+def test_a_state_written_in_place_counts_as_changed():
+    from tops import _rows
+    h = torch.randn(2, 3, 4)
+    x = torch.randn(2, 3, 4, requires_grad=True)
+    y = (x * h).sum()  # keeps h for the backward
+    assert _rows.state_target("step", h, h)[1] is h
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out = torch.zeros(2, 3, 4, requires_grad=True)
+    with pytest.raises(RuntimeError, match="state_out requires a gradient"):
+        _rows.state_target("step", h, out)
+    with torch.no_grad():
+        assert _rows.state_target("step", h, out)[1] is out
+    with torch.inference_mode():
+        t = torch.zeros(2, 3, 4)
+        assert _rows.state_target("step", t, t)[1] is t
