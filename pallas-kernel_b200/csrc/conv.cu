@@ -509,6 +509,7 @@ int by_type(int dtype, bool wide, int W, F f) {
 int check(const tops_gla_conv_args* a) {
   TOPS_CHECK_ARG(a != nullptr, "causal_conv: args is NULL");
   TOPS_CHECK_ARG(a->B >= 0 && a->T >= 0 && a->D > 0 && a->N >= 0, "causal_conv: negative or zero dimension");
+  if (a->B > kMaxRows || a->T > kMaxRows || a->D > kMaxChannels) return fail(TOPS_ERR_UNSUPPORTED, "causal_conv: too many rows or channels");
   if (a->W < 2 || a->W > 4) return fail(TOPS_ERR_UNSUPPORTED, "causal_conv: the kernel width must be 2, 3 or 4");
   TOPS_CHECK_ARG(dtype_known(a->dtype), "causal_conv: unknown dtype");
   TOPS_CHECK_ARG(a->w_dtype == a->dtype || a->w_dtype == TOPS_F32, "causal_conv: w_dtype must be dtype or TOPS_F32");

@@ -434,6 +434,8 @@ __global__ void __launch_bounds__(1024) k_qk_dw(int blocks, int K, int wdtype, c
 int check(const tops_gla_qk_norm_args* a) {
   TOPS_CHECK_ARG(a != nullptr, "qk_norm: args is NULL");
   TOPS_CHECK_ARG(a->B >= 0 && a->T >= 0 && a->H >= 0 && a->HK >= 0, "qk_norm: negative dimension");
+  if (a->B > kMaxRows || a->T > kMaxRows || a->H > kMaxChannels || a->HK > kMaxChannels)
+    return fail(TOPS_ERR_UNSUPPORTED, "qk_norm: too many rows or heads");
   if (a->K < 1 || a->K > 256) return fail(TOPS_ERR_UNSUPPORTED, "qk_norm: heads must have 1 to 256 elements");
   TOPS_CHECK_ARG(dtype_known(a->dtype), "qk_norm: unknown dtype");
   TOPS_CHECK_ARG(a->w_dtype == a->dtype || a->w_dtype == TOPS_F32, "qk_norm: w_dtype must be dtype or TOPS_F32");

@@ -188,6 +188,8 @@ __device__ __forceinline__ SeqAt seq_at(const int32_t* __restrict__ cu, int N, i
   return q;
 }
 
+// rows and channels are counted in 32 bits; a tile may step past the last row
+constexpr int kMaxRows = INT32_MAX - 65535, kMaxChannels = 1 << 28;
 inline bool dtype_known(int d) { return d == TOPS_F32 || d == TOPS_BF16 || d == TOPS_F16; }
 inline int dtype_bytes(int d) { return d == TOPS_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

@@ -259,6 +259,7 @@ inline int check(const tops_gla_scan_args* a) {
   TOPS_CHECK_ARG(a != nullptr, "ssm_scan: args is NULL");
   TOPS_CHECK_ARG(a->B >= 0 && a->T >= 0 && a->D > 0 && a->S >= 0, "ssm_scan: negative or zero dimension");
   TOPS_CHECK_ARG(a->G > 0 && a->D % a->G == 0, "ssm_scan: D must be a multiple of G");
+  if (a->T > kMaxRows || a->D > kMaxChannels) return fail(TOPS_ERR_UNSUPPORTED, "ssm_scan: too many rows or channels");
   if (a->G > 65535) return fail(TOPS_ERR_UNSUPPORTED, "ssm_scan: at most 65535 groups");
   if (a->N < 1 || a->N > 64) return fail(TOPS_ERR_UNSUPPORTED, "ssm_scan: a channel must have 1 to 64 states");
   TOPS_CHECK_ARG(dtype_known(a->dtype), "ssm_scan: unknown dtype");

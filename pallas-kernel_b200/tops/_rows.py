@@ -53,6 +53,16 @@ def eager_grads(op: str, *grads) -> None:
             raise RuntimeError(f"{op} has no gradient for a batch of them (is_grads_batched, torch.func)")
 
 
+# The kernels count rows and channels in 32 bits (offsets in 64); a tile may step past the last row.
+MAX_ROWS, MAX_CHANNELS = 2 ** 31 - 2 ** 16, 2 ** 28
+
+
+def check_sizes(op: str, batch: int, rows: int, channels: int) -> None:
+    if batch > MAX_ROWS or rows > MAX_ROWS or channels > MAX_CHANNELS:
+        raise ValueError(f"{op}: at most {MAX_ROWS} batch entries and rows and {MAX_CHANNELS} channels or heads, "
+                         f"got {batch}, {rows} and {channels}")
+
+
 def check_cuda(op: str, first: torch.Tensor, **others) -> None:
     """``first`` and every other given tensor lie on one CUDA device."""
     if not first.is_cuda:

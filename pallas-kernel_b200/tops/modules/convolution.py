@@ -176,6 +176,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     op = "causal_conv1d"
     _rows.eager_only(op, x, weight, bias, initial_state)
     assert x.dim() == 3, f"{op}: expected x [B, T, D], got {tuple(x.shape)}"
+    _rows.check_sizes(op, *x.shape)
     weight = _weight2d(op, weight)
     N, cu = _rows.sequences(op, cu_seqlens, x.shape[0], x.shape[1], x.device)
     _check(op, x, weight, bias, activation, x.shape[2], initial_state, (N,))
@@ -198,6 +199,7 @@ def causal_conv1d_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     assert x.dim() == 2, f"{op}: expected x [B, D], got {tuple(x.shape)}"
     weight = _weight2d(op, weight)
     B, D = x.shape
+    _rows.check_sizes(op, B, 1, D)
     _check(op, x, weight, bias, activation, D, state, (B,))
     _rows.no_grad_only(op, "causal_conv1d", x, state, weight, bias)
     x = _rows.rows(x)

@@ -100,6 +100,8 @@ def _check(op, q, k, q_weight, k_weight, cos, sin, positions):
     assert (cos is None) == (sin is None), f"{op}: cos and sin come together"
     if cos is None:
         return q_weight, k_weight, None, None, None
+    if cos.shape[0] > _rows.MAX_ROWS:
+        raise ValueError(f"{op}: at most {_rows.MAX_ROWS} positions in the tables, got {cos.shape[0]}")
     if cos.get_device() != dev or sin.get_device() != dev or (positions is not None and positions.get_device() != dev):
         _rows.check_cuda(op, q, cos=cos, sin=sin, positions=positions)
     R = 2 * cos.shape[-1]
@@ -141,7 +143,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     op = "qk_norm_rotary"
     _rows.eager_only(op, q, k, q_weight, k_weight, cos, sin)
     assert q.dim() == 4 and k.dim() == 4, f"{op}: expected q [B, T, H, K] and k [B, T, HK, K]"
-    B, T, _, K = q.shape
+    B, T, H, K = q.shape
+    _rows.check_sizes(op, B, T, H + k.shape[2])
     if not 1 <= K <= MAX_HEAD:
         raise ValueError(f"{op}: heads must have 1 to {MAX_HEAD} elements, got {K}")
     q_weight, k_weight, cos, sin, positions = _check(op, q, k, q_weight, k_weight, cos, sin, positions)

@@ -7,6 +7,7 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
 
 PKG = Path(__file__).resolve().parents[1] / "pallas-kernel_b200"
 
@@ -59,3 +60,26 @@ def test_scan_states_at_any_place(C):
         assert ("aligned" not in L.tops_gla_last_error().decode()) == ok
         assert L.tops_gla_ssm_scan_step(ctypes.byref(at(1, N, ht)), None) == -1
         assert "required" in L.tops_gla_last_error().decode()
+
+
+def test_sizes_past_32_bits_are_refused(C):
+    """A row count that wraps would leave most of the output unwritten."""
+    from tops.modules import causal_conv1d, causal_conv1d_step, qk_norm_rotary
+    from tops.ops.ssm import selective_scan, selective_scan_step
+    z = lambda *s: torch.zeros([1] * len(s)).expand(*s)  # noqa: E731
+    n, A, D = 2 ** 32 + 8, z(1, 4), 2 ** 32 + 8
+    for f in (lambda: causal_conv1d(z(1, n, 1), z(1, 4)), lambda: causal_conv1d(z(n, 1, 1), z(1, 4)),
+              lambda: causal_conv1d_step(z(n, 1), z(n, 1, 3), z(1, 4)),
+              lambda: selective_scan(z(1, n, 1), z(1, n, 1), A, z(1, n, 4), z(1, n, 4)),
+              lambda: selective_scan(z(1, 1, D), z(1, 1, D), z(D, 4), z(1, 1, 4), z(1, 1, 4)),
+              lambda: selective_scan_step(z(n, 1), z(n, 1), A, z(n, 4), z(n, 4), z(n, 1, 4)),
+              lambda: qk_norm_rotary(z(1, n, 1, 2), z(1, n, 1, 2)), lambda: qk_norm_rotary(z(1, 1, n, 2), z(1, 1, 1, 2))):
+        with pytest.raises(ValueError, match="at most"):
+            f()
+    big = 2 ** 31 - 1
+    for name, a in (("tops_gla_causal_conv_fwd", C.ConvArgs(B=1, T=big, D=8, W=4, N=1, dtype=C.BF16, w_dtype=C.BF16)),
+                    ("tops_gla_causal_conv_fwd", C.ConvArgs(B=1, T=1, D=big, W=4, N=1, dtype=C.BF16, w_dtype=C.BF16)),
+                    ("tops_gla_ssm_scan_fwd", C.ScanArgs(B=1, T=big, D=8, N=4, G=1, S=1, dtype=C.BF16)),
+                    ("tops_gla_qk_norm_rotary_fwd", C.QKNormArgs(B=1, T=big, H=1, HK=1, K=8, dtype=C.BF16, w_dtype=C.BF16))):
+        assert getattr(C.lib(), name)(ctypes.byref(a), None) == -2, name
+        assert "too many" in C.lib().tops_gla_last_error().decode()
