@@ -46,6 +46,32 @@ def test_scan_rows_behind_the_last_sequence_in_segments():
         assert not v[:, 433:].any()
 
 
+def test_scan_far_states_of_varied_steps():
+    """Small steps that differ from row to row, so that what the exponentials are off by on average adds up over a
+    state's memory while their roundings do not."""
+    g = torch.Generator().manual_seed(47)
+    T, ch, N = 4096, 32, 16
+    rn = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    t = {"x": rn(1, T, ch), "dt": -6.9 + rn(1, T, ch) / 2, "B": rn(1, T, 1, N), "C": rn(1, T, 1, N), "z": None,
+         "A": -torch.arange(1, N + 1.0).expand(ch, N).contiguous(), "D": None, "bias": None, "h0": None}
+    dout = rn(1, T, ch)
+    r = scan_ref(*(_dbl(t[k]) for k in NAMES), True, None, _dbl(dout), None)
+    c = {k: None if v is None else v.cuda().requires_grad_() for k, v in t.items()}
+    y, ht = _call(c, True, None)
+    names = ("x", "dt", "A", "B", "C")
+    got = dict(zip(names, torch.autograd.grad(y, [c[k] for k in names], dout.cuda())))
+    # A state that forgets within M rows weighs an error of k rows back by exp(-k / M): errors of one sign e a row come
+    # to e M / sqrt(2), rounded ones of 2^-24 a row to 2^-24 sqrt(M / 2).  M = 1000 / n for A = -n; outputs mix all n
+    # and their smallest M, 1000, bounds them: 2e-9 * 707 + 2^-24 * 22, and what the rounded steps add.
+    for name, v, want in (("out", y, r["out"][0]), ("ht", ht, r["ht"][0]), *((f"d{k}", got[k], r[f"d{k}"][0]) for k in names)):
+        rel = ((v.double().cpu() - want).norm() / want.norm()).item()
+        assert rel <= 3e-6, f"{name}: {rel:.2e}"
+    # A = -5 and below: M <= 200, 5e-9 * 141 + 2^-24 * 10 = 1.3e-6 and the sums' own roundings (an exponential that is
+    # 2e-8 off on average, as the hardware's is there, would give 2.8e-6)
+    err, size = (got["A"].double().cpu() - r["dA"][0])[:, 4:].norm(dim=0), r["dA"][0][:, 4:].norm(dim=0)
+    assert (err <= 1.5e-6 * size).all(), f"dA: {(err / size).max():.2e}"
+
+
 # -- norm and rotation ------------------------------------------------------------------------------------------
 
 
