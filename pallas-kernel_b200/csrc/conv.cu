@@ -6,7 +6,8 @@
 //
 // Nothing is reused but the W - 1 rows before a row, so HBM bounds it: a thread owns V channels (16 bytes; 8 in the
 // backward, whose sums need the registers) and walks down a strip of rows with the window in registers.  B8 T4096 D2048
-// bf16: forward 52 us = 5.2 TB/s, backward 104 us = 3.9 TB/s, the latter bound by instruction issue.
+// bf16, calls in a row: forward 57 us = 4.7 TB/s, backward 105 us = 3.8 TB/s and 115 with the parameters' sums.  The
+// backward fills no unit (HBM 46 %, issue 59 %): 128 registers leave 14 warps an SM, too few to cover each other's waits.
 #include <algorithm>
 
 #include "rowtypes.cuh"
@@ -552,7 +553,7 @@ void split(P& p, int v, int64_t threads_wanted, int most) {
 
 // Four blocks of 128 threads fill an SM's registers: strips that make one wave of them (forward) or two (backward), as
 // far as the cap lets them (23 packed prompts of 9973 rows: 22 -> 18 us against strips of 8; backward B8 T4096 D2048: 1024
-// threads an SM 108 us, 512: 114, 1536: 116).
+// threads an SM 108 us, 512: 114, 1536: 116, each between events of its own, which add some 3 us).
 constexpr int64_t kFwdThreads = 148 * 512, kBwdThreads = 148 * 1024;
 
 }  // namespace conv

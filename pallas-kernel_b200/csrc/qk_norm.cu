@@ -8,7 +8,8 @@
 // Nothing is reused between rows but the token's cosines and the weights, so HBM bounds it: a group of lanes owns a
 // token and walks its heads, V elements a lane.  The heads' vectors come through a ring in shared memory, several heads
 // ahead of their use and without registers; a rotated element's partner is read there from the other lane's column.
-// 32768 tokens, 16 + 4 heads of 128 bf16: forward 66 us = 5.1 TB/s, backward 120 us = 4.2 TB/s.
+// 32768 tokens, 16 + 4 heads of 128 bf16, calls in a row: forward 70 us = 4.8 TB/s (issue 76 %), backward 120 us =
+// 4.2 TB/s and 128 with the weights' sums (issue 65 %, HBM 48 %: 112 registers leave it 15 warps an SM).
 #include <algorithm>
 
 #include "rowtypes.cuh"

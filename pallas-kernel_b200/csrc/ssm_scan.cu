@@ -5,8 +5,9 @@ namespace tops {
 namespace ssm {
 
 // SUM: the first pass over a segment (its state from zero and the sum of delta) instead of its output.
-// B4 T2048 D4096 N16 bf16: 284 us at 512 blocks = 1.9e12 exponentials a second of 4.6e12; B1 T8191 in segments 228 us
-// and 152 us for the first pass.  64 or 256 threads a block: 295, 320 us; 4 rows in flight: 311.
+// B4 T2048 D4096 N16 bf16: 286 us at 512 blocks = 1.9e12 exponentials a second of 4.6e12 (266 where no states are
+// saved); B1 T8191 in segments 230 us and 155 us for the first pass.  64 or 256 threads a block: 295, 320 us; 4 rows in
+// flight: 311.
 constexpr int kFwdThreads = 128;
 
 template <typename T, int LN, int NT, bool VAR, bool SUM>

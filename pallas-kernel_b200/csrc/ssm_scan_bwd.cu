@@ -53,9 +53,9 @@ constexpr size_t bwd_smem() {
 
 // One segment, tile by tile from its end.  The states of kBwdPart rows at a time are computed again from the saved state
 // before them and kept in registers with their decays (eight rows spilled: 1088 against 1004 us); what the tile's outputs
-// need of the inputs stays packed as it came, the rest is read back from shared memory.  B4 T2048 D4096 N16 bf16: 925 us
-// at 256 blocks, 800 us for the same work in many more blocks; bound by instruction issue and the shared-memory pipe
-// (33 instructions and 0.28 wavefronts an element, of which the folds are 10 and 0.08).
+// need of the inputs stays packed as it came, the rest is read back from shared memory.  B4 T2048 D4096 N16 bf16: 930 us
+// at 256 blocks, 800 us for the same work in many more blocks.  No unit is full: issue 55 %, the shared-memory pipe 60 %
+// (33 instructions and 0.28 wavefronts an element, of which the folds are 10 and 0.08), 14 warps an SM.
 template <typename T, int LN, int NT, bool VAR>
 __global__ void __launch_bounds__(kBwdThreads, 2) k_scan_bwd(const P p) {
   constexpr int TS = kBwdRows, HALF = kBwdPart, DB = kBwdThreads / LN, NP = LN * NT, QC = DB / 4, NH = NT / 2;

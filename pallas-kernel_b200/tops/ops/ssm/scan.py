@@ -4,7 +4,7 @@
     h_t = exp(delta_t A[d, n]) h_{t-1} + delta_t x_t B_t[n]
     y_t = sum_n C_t[n] h_t + D x_t,    out = y silu(z)
 
-The forward, the backward and the single-token step run in ``ssm_scan.cu``
+The forward and the single-token step run in ``ssm_scan.cu``, the backward in ``ssm_scan_bwd.cu``
 (``tops_gla_ssm_scan_*``): fp32 arithmetic and states on fp32, bf16 or fp16 tensors.
 """
 from __future__ import annotations
@@ -138,8 +138,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         cu_seqlens: [S + 1] offsets of S sequences packed along T (batch size 1).  Offsets on the GPU are
             not read by the host (capturable); rows behind the last sequence give zeros.
     x, dt, z, B and C may be slices of wider tensors (dense channels).  A, D, dt_bias and states are
-    used in fp32.  Gradients flow to every tensor, also from the final state.  Eager calls only: tracing,
-    ``torch.func`` and forward mode are refused.
+    used in fp32.  Gradients flow to every tensor, also from the final state; for them the call keeps a state of
+    every eighth row, N / 2 bytes a row and channel.  Eager calls only: tracing, ``torch.func`` and forward mode
+    are refused.
     """
     op = "selective_scan"
     if _rows.watched():

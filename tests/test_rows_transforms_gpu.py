@@ -214,6 +214,14 @@ def test_backwards_refuse_what_they_cannot_follow():
             torch.autograd.grad(y, X, dy[None], is_grads_batched=True)
 
 
+def test_operators_inside_compiled_callers():
+    """The graph breaks at the operator, which runs as it does alone."""
+    for name, (f, x) in _calls().items():
+        with torch.no_grad():
+            want = f(x) * 2
+            assert torch.equal(torch.compile(lambda t, f=f: f(t) * 2, backend="eager")(x), want), name
+
+
 # -- second derivatives of the convolution ----------------------------------------------------------------------
 
 
