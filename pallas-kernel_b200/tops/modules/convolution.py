@@ -222,8 +222,8 @@ class ShortConvolution(nn.Module):
     tops/modules/convolution.py; torch gold tests/src/modules/convolution.py); the decode cache holds the
     last ``kernel_size - 1`` inputs of each sequence.  CUDA tensors of a kernel's dtype and width
     (``kernel_size`` 2 to 4) run on ``causal_conv1d``, packed sequences (``cu_seqlens``) there only;
-    the rest (CPU tensors, other widths, an autocast dtype other than x's; tracing and compiling, ``torch.func``,
-    forward mode, dispatch modes, tensor subclasses) is torch's conv1d."""
+    the rest (CPU tensors, other widths, an autocast dtype other than x's; without packing also tracing and
+    compiling, ``torch.func``, forward mode, dispatch modes, tensor subclasses) is torch's conv1d."""
 
     def __init__(self, hidden_size: int, kernel_size: int = 4, bias: bool = False, activation: str | None = "silu"):
         super().__init__()
@@ -233,23 +233,24 @@ class ShortConvolution(nn.Module):
         nn.init.kaiming_uniform_(self.weight, a=5 ** 0.5)
         self.activation = activation
 
-    def _on_kernel(self, x, cache):
-        if torch.compiler.is_compiling() or not x.is_cuda or x.dtype not in _C._DTYPE or self.kernel_size not in KERNEL_WIDTHS:
+    def _on_kernel(self, x, cache, packed):
+        if not x.is_cuda or x.dtype not in _C._DTYPE or self.kernel_size not in KERNEL_WIDTHS:
             return False
-        if not _rows.plain(x, self.weight, self.bias, cache):
+        # packed rows have no other form: causal_conv1d says what it cannot follow
+        if not packed and (torch.compiler.is_compiling() or not _rows.plain(x, self.weight, self.bias, cache)):
             return False
         return not torch.is_autocast_enabled("cuda") or x.dtype == torch.get_autocast_dtype("cuda")
 
     def forward(self, x, cache=None, output_final_state=False, cu_seqlens=None):
-        if self._on_kernel(x, cache):
+        if self._on_kernel(x, cache, cu_seqlens is not None):
             act = self.activation if self.activation in ("silu", "swish") else None
             bias = None if self.bias is None else self.bias.to(x.dtype)
             y, state = causal_conv1d(x, self.weight.to(x.dtype), bias, act, None if cache is None else cache.to(x.dtype),
                                      output_final_state, cu_seqlens)
             return y, None if state is None else state.detach()
         if cu_seqlens is not None:
-            raise NotImplementedError("ShortConvolution: packed (cu_seqlens) inputs need the kernel: an eager call on a CUDA "
-                                      "tensor in float32, bfloat16 or float16 and a kernel_size of 2 to 4")
+            raise NotImplementedError("ShortConvolution: packed (cu_seqlens) inputs need the kernel: a CUDA tensor in "
+                                      "float32, bfloat16 or float16 and a kernel_size of 2 to 4")
         B, T, D = x.shape
         xt = x.transpose(1, 2)  # [B, D, T]
         prev = cache if cache is not None else x.new_zeros(B, D, self.kernel_size - 1)

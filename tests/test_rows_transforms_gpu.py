@@ -160,6 +160,38 @@ def test_short_convolution_sees_modes_and_compilers():
         _near("compiled", torch.compile(g, backend="eager")(x2.cuda())[0], c(x2.double())[0], SIZE)
 
 
+def test_packed_short_convolution_under_modes_and_compilers():
+    """Packed rows have the kernel alone: what only looks on does not keep them from it, what cannot follow it is told."""
+    from torch.utils.flop_counter import FlopCounterMode
+    g, _ = _pair()
+    x = torch.randn(1, 20, 24, device="cuda")
+    cu = torch.tensor([0, 7, 7, 20], dtype=torch.int32, device="cuda")
+    want, state = g(x, None, True, cu)
+    with FlopCounterMode(display=False):
+        y, s = g(x, None, True, cu)
+    assert torch.equal(y, want) and torch.equal(s, state)
+    with torch.no_grad():
+        y, s = torch.compile(g, backend="eager")(x, None, True, cu)
+        assert torch.equal(y, want) and torch.equal(s, state)
+        g.requires_grad_(False)  # a function's trace takes no parameter that does
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(lambda t: g(t, None, False, cu)[0], x, check_trace=False)
+        with pytest.raises(RuntimeError, match="torch.func"):
+            torch.vmap(lambda t: g(t, None, False, cu)[0])(x[None])
+
+
+def test_vmap_over_a_backward():
+    """A batch of gradients by torch.vmap around autograd.grad, as by is_grads_batched."""
+    g, c = _pair()
+    x, dy = torch.randn(2, 7, 24), torch.randn(3, 2, 7, 24)
+    got = []
+    for m, cast in ((g, lambda v: v.cuda()), (c, lambda v: v.double())):
+        X = cast(x).requires_grad_()
+        y, _ = m(X)
+        got.append(torch.vmap(lambda v, y=y, X=X: torch.autograd.grad(y, X, v, retain_graph=True)[0])(cast(dy)))
+    _near("dx", *got, SIZE)
+
+
 def _calls():
     """Every operator as a function of one tensor that requires nothing, with its argument."""
     from tops.modules import causal_conv1d, causal_conv1d_step, qk_norm_rotary
