@@ -83,3 +83,24 @@ def test_sizes_past_32_bits_are_refused(C):
                     ("tops_gla_qk_norm_rotary_fwd", C.QKNormArgs(B=1, T=big, H=1, HK=1, K=8, dtype=C.BF16, w_dtype=C.BF16))):
         assert getattr(C.lib(), name)(ctypes.byref(a), None) == -2, name
         assert "too many" in C.lib().tops_gla_last_error().decode()
+
+
+def test_launches_go_to_the_tensors_device(monkeypatch):
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+    from tops import _rows
+    at, calls = [0], []
+
+    @contextmanager
+    def device(d):
+        keep, at[0] = at[0], d
+        yield
+        at[0] = keep
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: at[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(_rows._C, "stream_of", lambda t: 100 + t.device)
+    monkeypatch.setattr(_rows._C, "call", lambda name, args, stream: calls.append((name, args, stream, at[0])))
+    for d in (0, 1):
+        _rows.launch("f", "args", SimpleNamespace(device=d, get_device=lambda d=d: d))
+    assert calls == [("f", "args", 100, 0), ("f", "args", 101, 1)] and at == [0]
